@@ -1,0 +1,67 @@
+// Operators on block-128 fp8 tensors.
+//
+// A block-128 tensor is a pair (q, scales): q e4m3 [rows, cols] with a row
+// pitch that is a multiple of 16 bytes from a 16-byte aligned base, scales
+// fp32 [rows, ceil(cols / 128)] without gaps. Element (r, c) stands for
+// q[r, c] * scales[r, c / 128]. The weights that restore_cast and push write
+// (scale amax / 448) have this form when cols is a multiple of 128;
+// quantize_block128 writes power-of-two scales.
+//
+// Every launcher checks pointers, pitches and sizes on the host and returns
+// cudaErrorInvalidValue without launching when they do not fit; all launches
+// go on the caller's stream and none allocate memory.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace ofld {
+namespace kern {
+
+enum class FloatType : int { kBf16 = 0, kFp16 = 1, kFp32 = 2 };
+
+// A row-major matrix: element (r, c) at ptr + r * ld + c (ld in elements).
+struct MatIn {
+    const void* ptr;
+    int64_t ld;
+};
+struct MatOut {
+    void* ptr;
+    int64_t ld;
+};
+struct Block128In {
+    const void* q;
+    int64_t ld;  // bytes
+    const float* scales;
+};
+struct Block128Out {
+    void* q;
+    int64_t ld;
+    float* scales;
+};
+
+cudaError_t quantize_block128(MatIn x, FloatType type, Block128Out out, int64_t rows, int64_t cols, cudaStream_t s);
+cudaError_t dequantize_block128(Block128In in, MatOut x, FloatType type, int64_t rows, int64_t cols, cudaStream_t s);
+
+// h = silu(gate) * up; gate and up are also kept as block-128 tensors.
+cudaError_t swiglu_forward(MatIn gate, MatIn up, FloatType type, MatOut h, Block128Out kept_gate,
+                           Block128Out kept_up, int64_t rows, int64_t cols, cudaStream_t s);
+// Gradients at the kept values.
+cudaError_t swiglu_backward(MatIn dh, FloatType type, Block128In kept_gate, Block128In kept_up, MatOut dgate,
+                            MatOut dup, int64_t rows, int64_t cols, cudaStream_t s);
+
+// y[m, n] = x w^T (+ bias[n], may be null), x [m, k] and w [n, k] block-128.
+cudaError_t matmul_block128(Block128In x, Block128In w, const void* bias, MatOut y, FloatType type, int64_t m,
+                            int64_t n, int64_t k, cudaStream_t s);
+// dx[m, k] = dy w, dy [m, n] bf16, w [n, k] block-128.
+cudaError_t matmul_input_grad(MatIn dy, Block128In w, MatOut dx, FloatType type, int64_t m, int64_t n, int64_t k,
+                              cudaStream_t s);
+// dw[n, k] = dy^T x, dy [m, n] bf16, x [m, k] block-128.
+cudaError_t matmul_weight_grad(MatIn dy, Block128In x, MatOut dw, FloatType type, int64_t m, int64_t n, int64_t k,
+                               cudaStream_t s);
+
+uint64_t block128_launch_count();
+
+}  // namespace kern
+}  // namespace ofld

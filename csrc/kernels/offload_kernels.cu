@@ -24,6 +24,7 @@
 #include <mutex>
 #include <set>
 
+#include "block128.h"
 #include "kernels.h"
 #include "timing.h"
 #include "ofld/chunk_hash.h"
@@ -910,7 +911,8 @@ int grid_for(uint64_t nbytes, int ctas, int dflt) {
 
 
 
-uint64_t launch_count() { return g_launches.load(std::memory_order_relaxed) + push_launch_count(); }
+uint64_t launch_count() { return g_launches.load(std::memory_order_relaxed) + push_launch_count() +
+                                  block128_launch_count(); }
 
 cudaError_t evict_hash(const void* src, void* dst, uint64_t nbytes, uint64_t* digests, cudaStream_t s, int ctas) {
     if (nbytes == 0) return cudaSuccess;

@@ -31,6 +31,7 @@ namespace py = pybind11;
 using namespace ofld;
 
 void bind_fabric(py::module_& m);  // fabric_bind.cpp
+void bind_block128(py::module_& m);  // block128_bind.cpp
 
 namespace {
 
@@ -819,4 +820,5 @@ PYBIND11_MODULE(_C, m) {
     });
     m.def("host_unregister", [](uint64_t ptr) { check(cudaHostUnregister(reinterpret_cast<void*>(ptr)), "cudaHostUnregister"); });
     bind_fabric(m);
+    bind_block128(m);
 }

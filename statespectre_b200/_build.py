@@ -35,10 +35,11 @@ COMMON = ["common/codec.cpp", "common/transport.cpp", "common/metrics.cpp", "com
 DAEMON = ["daemon/config.cpp", "daemon/daemon.cpp", "daemon/slots.cpp", "daemon/tiers.cpp",
           "daemon/nvme.cpp", "daemon/canonical.cpp", "daemon/rollout.cpp", "daemon/persist.cpp"]
 AGENT = ["agent/agent.cpp"]
-KERNELS = ["kernels/offload_kernels.cu", "kernels/weight_sync.cu", "kernels/hash_noalloc.cu"]
+KERNELS = ["kernels/offload_kernels.cu", "kernels/weight_sync.cu", "kernels/hash_noalloc.cu",
+           "kernels/block128.cu", "kernels/block128_matmul.cu"]
 KERNEL_HOST = ["kernels/timing.cpp"]
 FABRIC = ["fabric/fabric.cpp", "fabric/vmm.cpp"]
-MODULE = ["python/module.cpp", "python/fabric_bind.cpp"]
+MODULE = ["python/module.cpp", "python/fabric_bind.cpp", "python/block128_bind.cpp"]
 
 ARCH = "-gencode arch=compute_100a,code=sm_100a"
 SANITIZERS = {

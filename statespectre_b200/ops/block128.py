@@ -1,0 +1,356 @@
+"""Operators on fp8 block-128 tensors.
+
+A block-128 tensor is the pair ``(q, scales)`` that ``handle.restore(cast="fp8_block128")`` and
+``RolloutWeights.get`` return: ``q`` holds e4m3 values, ``scales`` one fp32 factor for each 128 consecutive
+values of a row, and the pair stands for ``q * scale``. A row whose length is no multiple of 128 ends in a
+shorter block of its own, and rows of ``q`` start on 16-byte boundaries (a pair laid out otherwise is copied).
+
+* ``quantize`` / ``dequantize``: an activation to 8 bits and back, with power-of-two scales
+* ``linear``: ``x @ w.T`` on the fp8 tensor cores; with gradients, the quantised operands of the forward
+  product are the only activations and weights kept for the backward pass
+* ``linear_input_grad`` / ``linear_weight_grad``: the two products of that backward pass
+* ``swiglu`` (and its two passes): the gated activation, keeping its inputs in 8 bits
+
+Everything runs on the current stream of the tensors' device and can be captured into a CUDA graph.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from .._native import native
+
+Block128 = Tuple[torch.Tensor, torch.Tensor]
+
+BLOCK = 128
+_FP8 = torch.float8_e4m3fn
+_TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _type(dtype: torch.dtype, what: str) -> int:
+    try:
+        return _TYPE[dtype]
+    except KeyError:
+        raise ValueError(f"{what} must be bfloat16, float16 or float32; got {dtype}") from None
+
+
+def _on_gpu(t, what: str) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} must be a tensor; got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{what} must be a CUDA tensor")
+    return t
+
+
+def _same_device(dev: torch.device, **tensors) -> None:
+    for what, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what} is on {t.device}, the first operand on {dev}")
+
+
+def _matrix(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
+    """(2-D form with unit column stride, rows, cols, pitch): a view where the strides allow one."""
+    if t.dim() == 0:
+        raise ValueError(f"{what} must have at least one dimension")
+    cols = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(t.numel() // cols if cols else 0, cols)
+    rows = t.shape[0]
+    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
+        t = t.contiguous()
+    return t, rows, cols, t.stride(0) if rows > 1 else cols
+
+
+def _tiled(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
+    """``_matrix`` whose base and pitch are multiples of 16 bytes, as the tile copies need: a copy if they are not."""
+    t, rows, cols, ld = _matrix(t, what)
+    per = 16 // t.element_size()
+    pitch = -(-cols // per) * per
+    if rows == 1:
+        ld = pitch
+    if ld % per or t.data_ptr() % 16:
+        p = torch.empty((rows, pitch), dtype=t.dtype, device=t.device)[:, :cols]
+        t, ld = p.copy_(t), pitch
+    return t, rows, cols, ld
+
+
+def _pair(p, what: str):
+    """(q, scales, rows, cols, pitch) of a block-128 pair."""
+    if not isinstance(p, (tuple, list)) or len(p) != 2:
+        raise TypeError(f"{what} must be a (q, scales) pair")
+    q, scales = _on_gpu(p[0], f"{what}: q"), _on_gpu(p[1], f"{what}: scales")
+    if q.dtype != _FP8:
+        raise ValueError(f"{what}: q must be float8_e4m3fn; got {q.dtype}")
+    if scales.dtype != torch.float32:
+        raise ValueError(f"{what}: scales must be float32; got {scales.dtype}")
+    _same_device(q.device, scales=scales)
+    q, rows, cols, ld = _tiled(q, f"{what}: q")
+    if scales.numel() != rows * -(-cols // BLOCK):
+        raise ValueError(f"{what}: {tuple(scales.shape)} scales do not fit {rows} rows of {cols} values: one for "
+                         f"each {BLOCK} values of a row")
+    return q, scales.contiguous(), rows, cols, ld
+
+
+def _stream(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+class _on:
+    """The device as the current one, for as long as it takes; costs nothing when it already is."""
+
+    def __init__(self, dev: torch.device):
+        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _empty_pair(shape, dev: torch.device):
+    """Uninitialised (q, scales) for values of `shape`, and q's pitch."""
+    cols = shape[-1]
+    pitch = -(-cols // 16) * 16
+    q = torch.empty((*shape[:-1], pitch), dtype=_FP8, device=dev)
+    if pitch != cols:
+        q = q[..., :cols]
+    return (q, torch.empty((*shape[:-1], -(-cols // BLOCK)), dtype=torch.float32, device=dev)), pitch
+
+
+def quantize(x: torch.Tensor) -> Block128:
+    """``x`` [..., cols] (bfloat16, float16 or float32) in 8 bits: ``(q, scales)``, ``q`` [..., cols] and one scale
+    per 128 values, [..., ceil(cols / 128)].
+
+    The scale is the smallest power of two (at least 2^-117) that brings a block within e4m3's 448, 1 for a block
+    of zeros, so the only rounding is e4m3's (to nearest, ties to even). A value that is not finite becomes NaN and
+    does not count in its block's scale."""
+    x = _on_gpu(x.detach() if isinstance(x, torch.Tensor) else x, "x")
+    code = _type(x.dtype, "x")
+    shape = x.shape
+    x, rows, cols, ld = _matrix(x, "x")
+    (q, scales), pitch = _empty_pair(shape, x.device)
+    with _on(x.device):
+        native().k_quantize_block128(x.data_ptr(), ld, code, q.data_ptr(), pitch, scales.data_ptr(), rows, cols,
+                                     _stream(x.device))
+    return q, scales
+
+
+def dequantize(x: Block128, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values that a pair stands for, rounded to ``dtype`` (no rounding in bfloat16 and float32 where
+    ``quantize`` made the pair)."""
+    code = _type(dtype, "dtype")
+    q, scales, rows, cols, ld = _pair(x, "x")
+    out = torch.empty(x[0].shape, dtype=dtype, device=q.device)
+    with _on(q.device):
+        native().k_dequantize_block128(q.data_ptr(), ld, scales.data_ptr(), out.data_ptr(), cols, code, rows, cols,
+                                       _stream(q.device))
+    return out
+
+
+def _product(xp, wp, bias, out_dtype, lead) -> torch.Tensor:
+    xq, xs, m, k, ldx = xp
+    wq, ws, n, kw, ldw = wp
+    if k != kw:
+        raise ValueError(f"x has {k} columns, the weight {kw}")
+    dev = xq.device
+    _same_device(dev, weight=wq, bias=bias)
+    if bias is not None:
+        if bias.shape != (n,):
+            raise ValueError(f"bias must have shape ({n},); got {tuple(bias.shape)}")
+        if bias.dtype != out_dtype:
+            raise ValueError(f"bias must be {out_dtype} like the result; got {bias.dtype}")
+        bias = bias.contiguous()
+    y = torch.empty((*lead, n), dtype=out_dtype, device=dev)
+    if k == 0:
+        return y.zero_() if bias is None else y.copy_(bias.expand_as(y))
+    with _on(dev):
+        native().k_matmul_block128(xq.data_ptr(), ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(),
+                                   0 if bias is None else bias.data_ptr(), y.data_ptr(), n, _TYPE[out_dtype], m, n, k,
+                                   _stream(dev))
+    return y
+
+
+def linear(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None,
+           out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``x @ weight.T (+ bias)``: ``x`` [..., k] is quantised (as ``quantize`` does) and multiplied in 8 bits with
+    fp32 sums. ``weight`` is a pair [n, k] as restored or pushed in fp8 (any scales), or a floating tensor [n, k],
+    which is quantised too. The result has ``x``'s dtype unless ``out_dtype`` says otherwise.
+
+    With gradients (``x`` bfloat16), the backward pass uses the quantised operands: ``dx = dy @ w`` and
+    ``dw = dy.T @ x`` at the values that the forward product saw, and nothing else is kept. The quantisation
+    itself passes gradients through unchanged."""
+    _on_gpu(x, "x")
+    _type(x.dtype, "x")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    _type(out_dtype, "out_dtype")
+    if isinstance(weight, torch.Tensor):
+        _on_gpu(weight, "weight")
+        _type(weight.dtype, "weight")
+        wanted = x.requires_grad or weight.requires_grad
+    else:
+        wanted = x.requires_grad
+    if bias is not None:
+        _on_gpu(bias, "bias")
+        wanted = wanted or bias.requires_grad
+    if wanted and torch.is_grad_enabled():
+        if x.dtype != torch.bfloat16 or out_dtype != torch.bfloat16:
+            raise ValueError("linear with gradients needs bfloat16 activations")
+        if isinstance(weight, torch.Tensor):
+            return _Linear.apply(x, weight, bias, None)
+        return _Linear.apply(x, None, bias, weight)
+    return _forward(x, weight, bias, out_dtype)[0]
+
+
+def _weight_pair(weight):
+    q = weight if isinstance(weight, torch.Tensor) else weight[0] if isinstance(weight, (tuple, list)) else None
+    if isinstance(q, torch.Tensor) and q.dim() != 2:
+        raise ValueError(f"weight must have two dimensions; got {q.dim()}")
+    return _pair(quantize(weight) if isinstance(weight, torch.Tensor) else weight, "weight")
+
+
+def _forward(x, weight, bias, out_dtype):
+    wp = _weight_pair(weight)
+    if x.dim() == 0 or x.shape[-1] != wp[3]:
+        raise ValueError(f"x has shape {tuple(x.shape)}, the weight {wp[3]} columns")
+    xp = _pair(quantize(x), "x")
+    return _product(xp, wp, bias, out_dtype, x.shape[:-1]), xp, wp
+
+
+def _gradient(dy: torch.Tensor, other: Block128, what: str):
+    _on_gpu(dy, "dy")
+    if dy.dtype != torch.bfloat16:
+        raise ValueError(f"dy must be bfloat16; got {dy.dtype}")
+    p = _pair(other, what)
+    _same_device(dy.device, **{what: p[0]})
+    return _tiled(dy.detach(), "dy"), p
+
+
+def linear_input_grad(dy: torch.Tensor, weight: Block128, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``dy @ w`` for ``dy`` [..., n] (bfloat16) and a pair ``weight`` [n, k]: [..., k]. Each weight is brought to
+    bfloat16 for the tensor cores, exactly when its scale is a power of two; sums are in fp32."""
+    code = _type(out_dtype, "out_dtype")
+    (d, m, n, ldd), (q, scales, rows, k, ld) = _gradient(dy, weight, "weight")
+    if rows != n or weight[0].dim() != 2:
+        raise ValueError(f"dy has {n} columns, the weight shape {tuple(weight[0].shape)}")
+    dx = torch.empty((*dy.shape[:-1], k), dtype=out_dtype, device=d.device)
+    if n == 0:
+        return dx.zero_()
+    with _on(d.device):
+        native().k_matmul_input_grad(d.data_ptr(), ldd, q.data_ptr(), ld, scales.data_ptr(), dx.data_ptr(), k, code,
+                                     m, n, k, _stream(d.device))
+    return dx
+
+
+def linear_weight_grad(dy: torch.Tensor, x: Block128, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``dy.T @ x`` for ``dy`` [..., n] (bfloat16) and the kept pair ``x`` [..., k]: [n, k], summed over all rows in
+    fp32. The kept values go to the tensor cores as bfloat16, exactly when their scales are powers of two."""
+    code = _type(out_dtype, "out_dtype")
+    (d, m, n, ldd), (q, scales, rows, k, ld) = _gradient(dy, x, "x")
+    if rows != m:
+        raise ValueError(f"dy has {m} rows, x {rows}")
+    dw = torch.empty((n, k), dtype=out_dtype, device=d.device)
+    if m == 0:
+        return dw.zero_()
+    with _on(d.device):
+        native().k_matmul_weight_grad(d.data_ptr(), ldd, q.data_ptr(), ld, scales.data_ptr(), dw.data_ptr(), k, code,
+                                      m, n, k, _stream(d.device))
+    return dw
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, pair):
+        y, xp, wp = _forward(x, pair if weight is None else weight, bias, torch.bfloat16)
+        need_dw = weight is not None and weight.requires_grad
+        ctx.save_for_backward(*(xp[:2] if need_dw else (None, None)),
+                              *(wp[:2] if x.requires_grad else (None, None)))
+        ctx.x_shape = x.shape
+        ctx.weight_dtype = None if weight is None else weight.dtype
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        xq, xs, wq, ws = ctx.saved_tensors
+        dx = dw = db = None
+        if ctx.needs_input_grad[0]:
+            dx = linear_input_grad(dy, (wq, ws)).view(ctx.x_shape)
+        if ctx.needs_input_grad[1]:
+            dw = linear_weight_grad(dy, (xq, xs), ctx.weight_dtype)
+        if ctx.needs_input_grad[2]:
+            db = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32).to(ctx.bias_dtype)
+        return dx, dw, db, None
+
+
+def swiglu_forward(gate: torch.Tensor, up: torch.Tensor):
+    """``silu(gate) * up`` and what its backward pass keeps: ``(h, (kept_gate, kept_up))``, two pairs as ``quantize``
+    makes them. ``h`` is computed from the unquantised inputs."""
+    gate, up = (t.detach() if isinstance(t, torch.Tensor) else t for t in (gate, up))
+    _on_gpu(gate, "gate")
+    _on_gpu(up, "up")
+    code = _type(gate.dtype, "gate")
+    if up.dtype != gate.dtype or up.shape != gate.shape:
+        raise ValueError(f"up ({tuple(up.shape)}, {up.dtype}) must match gate ({tuple(gate.shape)}, {gate.dtype})")
+    dev = gate.device
+    _same_device(dev, up=up)
+    shape = gate.shape
+    g, rows, cols, ldg = _matrix(gate, "gate")
+    u, _, _, ldu = _matrix(up, "up")
+    h = torch.empty(shape, dtype=gate.dtype, device=dev)
+    kg, pitch = _empty_pair(shape, dev)
+    ku, _ = _empty_pair(shape, dev)
+    with _on(dev):
+        native().k_swiglu_forward(g.data_ptr(), ldg, u.data_ptr(), ldu, code, h.data_ptr(), cols, kg[0].data_ptr(),
+                                  kg[1].data_ptr(), ku[0].data_ptr(), ku[1].data_ptr(), pitch, rows, cols,
+                                  _stream(dev))
+    return h, (kg, ku)
+
+
+def swiglu_backward(dh: torch.Tensor, kept) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(dgate, dup)`` from ``dh`` and what ``swiglu_forward`` kept: the gradients of ``silu(gate) * up`` at the
+    kept values, in ``dh``'s dtype."""
+    _on_gpu(dh, "dh")
+    code = _type(dh.dtype, "dh")
+    if not isinstance(kept, (tuple, list)) or len(kept) != 2:
+        raise TypeError("kept must be the two pairs that swiglu_forward returned")
+    gq, gs, rows, cols, ldg = _pair(kept[0], "kept gate")
+    uq, us, rows_u, cols_u, ldu = _pair(kept[1], "kept up")
+    d, rows_d, cols_d, ldd = _matrix(dh.detach(), "dh")
+    if (rows, cols) != (rows_u, cols_u) or (rows, cols) != (rows_d, cols_d):
+        raise ValueError(f"dh has shape {tuple(dh.shape)}, the kept pairs {tuple(kept[0][0].shape)} and "
+                         f"{tuple(kept[1][0].shape)}")
+    dev = d.device
+    _same_device(dev, gate=gq, up=uq)
+    dg, du = (torch.empty(dh.shape, dtype=dh.dtype, device=dev) for _ in range(2))
+    with _on(dev):
+        native().k_swiglu_backward(d.data_ptr(), ldd, code, gq.data_ptr(), ldg, gs.data_ptr(), uq.data_ptr(), ldu,
+                                   us.data_ptr(), dg.data_ptr(), du.data_ptr(), cols, rows, cols, _stream(dev))
+    return dg, du
+
+
+class _SwiGLU(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, up):
+        h, (kg, ku) = swiglu_forward(gate, up)
+        ctx.save_for_backward(*kg, *ku)
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        gq, gs, uq, us = ctx.saved_tensors
+        return swiglu_backward(dh, ((gq, gs), (uq, us)))
+
+
+def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """``silu(gate) * up``; with gradients, the inputs are kept in 8 bits (2 bytes a pair of values instead of 4 or
+    8) and the backward pass takes its derivatives at the kept values."""
+    if torch.is_grad_enabled() and (getattr(gate, "requires_grad", False) or getattr(up, "requires_grad", False)):
+        return _SwiGLU.apply(gate, up)
+    return swiglu_forward(gate, up)[0]
