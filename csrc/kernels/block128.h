@@ -63,5 +63,10 @@ cudaError_t matmul_weight_grad(MatIn dy, Block128In x, MatOut dw, FloatType type
 
 uint64_t block128_launch_count();
 
+// Code of the first bounded wait that ran out in a product kernel on
+// `device` (its result is then incomplete); 0 if none did. Host memory, read
+// without waiting for the device.
+uint32_t block128_error(int device);
+
 }  // namespace kern
 }  // namespace ofld

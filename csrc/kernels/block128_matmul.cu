@@ -105,14 +105,6 @@ QuantAt quant_at(const Block128In& t, int64_t cols) {
 
 }  // namespace
 
-cudaError_t matmul_block128(Block128In x, Block128In w, const void* bias, MatOut y, FloatType type, int64_t m,
-                            int64_t n, int64_t k, cudaStream_t s) {
-    if (!dims_ok(m, n, k) || k == 0) return cudaErrorInvalidValue;
-    if (m == 0 || n == 0) return cudaSuccess;
-    if (!q_ok(x, k) || !q_ok(w, k) || !y.ptr || y.ld < n) return cudaErrorInvalidValue;
-    return launch<false, false>(quant_at(x, k), quant_at(w, k), bias, y, type, m, n, k, s);
-}
-
 cudaError_t matmul_input_grad(MatIn dy, Block128In w, MatOut dx, FloatType type, int64_t m, int64_t n, int64_t k,
                               cudaStream_t s) {
     if (!dims_ok(m, n, k) || n == 0) return cudaErrorInvalidValue;

@@ -12,6 +12,16 @@ namespace {
 void check(cudaError_t e, const char* what) {
     if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
 }
+// A product kernel whose bounded wait ran out has left its result incomplete:
+// the calls after it say so.
+void check_product(cudaError_t e, const char* what) {
+    check(e, what);
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) return;  // nothing can have been launched
+    if (const uint32_t code = block128_error(dev))
+        throw std::runtime_error(std::string(what) + ": a product on this device gave up waiting (code " +
+                                 std::to_string(code) + "); results since then are not complete");
+}
 MatIn in(uint64_t p, int64_t ld) { return {reinterpret_cast<const void*>(p), ld}; }
 MatOut out(uint64_t p, int64_t ld) { return {reinterpret_cast<void*>(p), ld}; }
 Block128In qin(uint64_t q, int64_t ld, uint64_t s) {
@@ -25,6 +35,7 @@ cudaStream_t stream(uint64_t s) { return reinterpret_cast<cudaStream_t>(s); }
 }  // namespace
 
 void bind_block128(py::module_& m) {
+    m.def("block128_error", &block128_error);
     m.def("k_quantize_block128", [](uint64_t x, int64_t ldx, int type, uint64_t q, int64_t ldq, uint64_t sc,
                                     int64_t rows, int64_t cols, uint64_t s) {
         check(quantize_block128(in(x, ldx), FloatType(type), qout(q, ldq, sc), rows, cols, stream(s)),
@@ -52,18 +63,18 @@ void bind_block128(py::module_& m) {
     m.def("k_matmul_block128", [](uint64_t xq, int64_t ldx, uint64_t xs, uint64_t wq, int64_t ldw, uint64_t ws,
                                   uint64_t bias, uint64_t y, int64_t ldy, int type, int64_t mm, int64_t n, int64_t k,
                                   uint64_t s) {
-        check(matmul_block128(qin(xq, ldx, xs), qin(wq, ldw, ws), reinterpret_cast<const void*>(bias), out(y, ldy),
+        check_product(matmul_block128(qin(xq, ldx, xs), qin(wq, ldw, ws), reinterpret_cast<const void*>(bias), out(y, ldy),
                               FloatType(type), mm, n, k, stream(s)),
               "matmul_block128");
     });
     m.def("k_matmul_input_grad", [](uint64_t dy, int64_t lddy, uint64_t wq, int64_t ldw, uint64_t ws, uint64_t dx,
                                     int64_t lddx, int type, int64_t mm, int64_t n, int64_t k, uint64_t s) {
-        check(matmul_input_grad(in(dy, lddy), qin(wq, ldw, ws), out(dx, lddx), FloatType(type), mm, n, k, stream(s)),
+        check_product(matmul_input_grad(in(dy, lddy), qin(wq, ldw, ws), out(dx, lddx), FloatType(type), mm, n, k, stream(s)),
               "matmul_input_grad");
     });
     m.def("k_matmul_weight_grad", [](uint64_t dy, int64_t lddy, uint64_t xq, int64_t ldx, uint64_t xs, uint64_t dw,
                                      int64_t lddw, int type, int64_t mm, int64_t n, int64_t k, uint64_t s) {
-        check(matmul_weight_grad(in(dy, lddy), qin(xq, ldx, xs), out(dw, lddw), FloatType(type), mm, n, k, stream(s)),
+        check_product(matmul_weight_grad(in(dy, lddy), qin(xq, ldx, xs), out(dw, lddw), FloatType(type), mm, n, k, stream(s)),
               "matmul_weight_grad");
     });
 }

@@ -157,7 +157,7 @@ def test_quantize_writes_nothing_beside_its_rows():
 
 SHAPES = [(1, 128, 1), (1, 5120, 640), (2, 128, 129), (3, 384, 255), (7, 1792, 1003), (16, 256, 512), (17, 4096, 136),
           (33, 128, 40), (64, 1024, 384), (65, 640, 1000), (128, 512, 256), (129, 256, 257), (200, 3456, 130),
-          (256, 384, 512), (300, 2048, 777), (513, 128, 1025), (640, 1280, 2048)]
+          (256, 384, 512), (300, 2048, 777), (513, 128, 1025), (640, 1280, 2048), (1531, 896, 5001), (2100, 384, 3333)]
 
 
 @pytest.mark.parametrize("m,k,n", SHAPES)
