@@ -22,6 +22,7 @@
 #include <atomic>
 
 #include "block128.h"
+#include "block128_host.h"
 
 namespace ofld {
 namespace kern {
@@ -157,14 +158,17 @@ __device__ __forceinline__ Pos locate(const Shape& sh, uint32_t blk) {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     k_quantize(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq,
-               float* __restrict__ scales, Shape sh) {
+               float* __restrict__ scales, TileScales tiles, Shape sh) {
     FOR_BLOCKS(blk) {
         const Pos p = locate(sh, blk);
         float f[8], s;
         load8<T, VEC>(x + p.row * ldx, p.c, p.n, f);
         const uint2 v = quantize8(f, &s);
         store_q(q + p.row * ldq, p.c, p.n, v);
-        if ((threadIdx.x & 15) == 0 && blk < sh.total) scales[blk] = s;
+        if ((threadIdx.x & 15) == 0 && blk < sh.total) {
+            if (scales) scales[blk] = s;
+            if (tiles.words) tiles.words[tiles.at(p.row, p.b, sh.nb)] = __float_as_uint(s) >> 23;
+        }
     }
 }
 
@@ -249,9 +253,8 @@ size_t size_of(FloatType t) { return t == FloatType::kFp32 ? 4 : 2; }
 bool type_ok(FloatType t) { return t == FloatType::kBf16 || t == FloatType::kFp16 || t == FloatType::kFp32; }
 bool vec_ok(const void* p, int64_t ld, FloatType t) { return aligned16(p) && (ld * int64_t(size_of(t))) % 16 == 0; }
 bool mat_ok(const void* p, int64_t ld, int64_t cols) { return p && ld >= cols; }
-bool q_ok(const void* q, int64_t ld, const float* s, int64_t cols) {
-    return q && s && aligned16(q) && ld % 16 == 0 && ld >= cols;
-}
+bool q_ptr_ok(const void* q, int64_t ld, int64_t cols) { return q && aligned16(q) && ld % 16 == 0 && ld >= cols; }
+bool q_ok(const void* q, int64_t ld, const float* s, int64_t cols) { return s && q_ptr_ok(q, ld, cols); }
 
 // False when the sizes are out of range; an empty shape has total 0.
 bool make_shape(int64_t rows, int64_t cols, Shape* sh) {
@@ -282,15 +285,21 @@ void by_type(FloatType t, F f) {
 }  // namespace
 
 cudaError_t quantize_block128(MatIn x, FloatType type, Block128Out out, int64_t rows, int64_t cols, cudaStream_t s) {
+    if (rows > 0 && cols > 0 && !out.scales) return cudaErrorInvalidValue;
+    return quantize_for_tiles(x, type, out, TileScales{}, rows, cols, s);
+}
+
+cudaError_t quantize_for_tiles(MatIn x, FloatType type, Block128Out out, TileScales tiles, int64_t rows, int64_t cols,
+                               cudaStream_t s) {
     Shape sh;
     if (!make_shape(rows, cols, &sh) || !type_ok(type)) return cudaErrorInvalidValue;
     if (sh.total == 0) return cudaSuccess;
-    if (!mat_ok(x.ptr, x.ld, cols) || !q_ok(out.q, out.ld, out.scales, cols)) return cudaErrorInvalidValue;
+    if (!mat_ok(x.ptr, x.ld, cols) || !q_ptr_ok(out.q, out.ld, cols)) return cudaErrorInvalidValue;
     by_type(type, [&](auto t) {
         using T = decltype(t);
         auto* fn = vec_ok(x.ptr, x.ld, type) ? k_quantize<T, true> : k_quantize<T, false>;
         fn<<<grid(sh), kThreads, 0, s>>>(static_cast<const T*>(x.ptr), x.ld, static_cast<uint8_t*>(out.q), out.ld,
-                                         out.scales, sh);
+                                         out.scales, tiles, sh);
     });
     return launched();
 }

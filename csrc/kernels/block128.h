@@ -51,9 +51,13 @@ cudaError_t swiglu_forward(MatIn gate, MatIn up, FloatType type, MatOut h, Block
 cudaError_t swiglu_backward(MatIn dh, FloatType type, Block128In kept_gate, Block128In kept_up, MatOut dgate,
                             MatOut dup, int64_t rows, int64_t cols, cudaStream_t s);
 
-// y[m, n] = x w^T (+ bias[n], may be null), x [m, k] and w [n, k] block-128.
-cudaError_t matmul_block128(Block128In x, Block128In w, const void* bias, MatOut y, FloatType type, int64_t m,
-                            int64_t n, int64_t k, cudaStream_t s);
+// y[m, n] = x w^T (+ bias[n], may be null) for x [m, k], quantised on the way
+// into `kept` (its scales may be null: then only q is written), and w [n, k]
+// block-128. `work` holds at least linear_work_bytes(m, k), 16-byte aligned.
+uint64_t linear_work_bytes(int64_t m, int64_t k);
+cudaError_t linear_block128(MatIn x, FloatType xtype, Block128Out kept, void* work, uint64_t work_bytes, Block128In w,
+                            const void* bias, MatOut y, FloatType type, int64_t m, int64_t n, int64_t k,
+                            cudaStream_t s);
 // dx[m, k] = dy w, dy [m, n] bf16, w [n, k] block-128.
 cudaError_t matmul_input_grad(MatIn dy, Block128In w, MatOut dx, FloatType type, int64_t m, int64_t n, int64_t k,
                               cudaStream_t s);

@@ -109,14 +109,6 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
         "l"(m), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
-// Four bytes, zeros when !valid.
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
-}
-// Arrives once all earlier cp.async of this thread have landed.
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ---- clusters
@@ -192,6 +184,40 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
             "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
             : "memory");
 }
+// The same with a factor for each row of A and of B (e8m0, one byte a row).
+template <int CG>
+__device__ __forceinline__ void mma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scale_a,
+                                         uint32_t scale_b, bool add) {
+    if (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)), "r"(scale_a), "r"(scale_b)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)), "r"(scale_a), "r"(scale_b)
+            : "memory");
+}
+// Factors of 128 rows from shared memory (512 bytes: 16 bytes a lane, word j of
+// lane i for row 32 j + i) to four columns of tensor memory, for all four
+// groups of 32 lanes. Runs in order with this thread's products.
+template <int CG>
+__device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint32_t src) {
+    const uint64_t desc = uint64_t((src & 0x3ffff) >> 4) | uint64_t(1) << 16 | uint64_t(128 >> 4) << 32 | uint64_t(1) << 46;
+    if (CG == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+// One word in each of four columns of this warp's lanes.
+__device__ __forceinline__ void tmem_fill4(uint32_t addr, uint32_t v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(v) : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
 // The barrier (in a pair: the one at this offset of both CTAs) gets one
 // arrival when the tcgen05 operations issued so far by this thread are done.
 template <int CG>
@@ -250,6 +276,11 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t mn_stri
 __host__ __device__ constexpr uint32_t instr_desc(int m, int n, uint32_t fmt, bool a_mn, bool b_mn) {
     return 1u << 4 | fmt << 7 | fmt << 10 | uint32_t(a_mn) << 15 | uint32_t(b_mn) << 16 | uint32_t(n >> 3) << 17 |
            uint32_t(m >> 4) << 24;
+}
+
+// The one of products with factors: e4m3 operands, e8m0 factors in byte 0.
+__host__ __device__ constexpr uint32_t instr_desc_mxf8(int m, int n) {
+    return uint32_t(n >> 3) << 17 | 1u << 23 | uint32_t(m >> 4) << 24;
 }
 
 // ---- packed fp32 pairs

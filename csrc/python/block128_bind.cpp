@@ -60,12 +60,15 @@ void bind_block128(py::module_& m) {
                               out(du, ldd), rows, cols, stream(s)),
               "swiglu_backward");
     });
-    m.def("k_matmul_block128", [](uint64_t xq, int64_t ldx, uint64_t xs, uint64_t wq, int64_t ldw, uint64_t ws,
+    m.def("linear_work_bytes", &linear_work_bytes);
+    m.def("k_linear_block128", [](uint64_t x, int64_t ldx, int xtype, uint64_t xq, int64_t ldq, uint64_t xs,
+                                  uint64_t work, uint64_t work_bytes, uint64_t wq, int64_t ldw, uint64_t ws,
                                   uint64_t bias, uint64_t y, int64_t ldy, int type, int64_t mm, int64_t n, int64_t k,
                                   uint64_t s) {
-        check_product(matmul_block128(qin(xq, ldx, xs), qin(wq, ldw, ws), reinterpret_cast<const void*>(bias), out(y, ldy),
-                              FloatType(type), mm, n, k, stream(s)),
-              "matmul_block128");
+        check_product(linear_block128(in(x, ldx), FloatType(xtype), qout(xq, ldq, xs), reinterpret_cast<void*>(work),
+                                      work_bytes, qin(wq, ldw, ws), reinterpret_cast<const void*>(bias), out(y, ldy),
+                                      FloatType(type), mm, n, k, stream(s)),
+                      "linear_block128");
     });
     m.def("k_matmul_input_grad", [](uint64_t dy, int64_t lddy, uint64_t wq, int64_t ldw, uint64_t ws, uint64_t dx,
                                     int64_t lddx, int type, int64_t mm, int64_t n, int64_t k, uint64_t s) {

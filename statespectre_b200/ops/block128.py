@@ -152,29 +152,6 @@ def dequantize(x: Block128, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor
     return out
 
 
-def _product(xp, wp, bias, out_dtype, lead) -> torch.Tensor:
-    xq, xs, m, k, ldx = xp
-    wq, ws, n, kw, ldw = wp
-    if k != kw:
-        raise ValueError(f"x has {k} columns, the weight {kw}")
-    dev = xq.device
-    _same_device(dev, weight=wq, bias=bias)
-    if bias is not None:
-        if bias.shape != (n,):
-            raise ValueError(f"bias must have shape ({n},); got {tuple(bias.shape)}")
-        if bias.dtype != out_dtype:
-            raise ValueError(f"bias must be {out_dtype} like the result; got {bias.dtype}")
-        bias = bias.contiguous()
-    y = torch.empty((*lead, n), dtype=out_dtype, device=dev)
-    if k == 0:
-        return y.zero_() if bias is None else y.copy_(bias.expand_as(y))
-    with _on(dev):
-        native().k_matmul_block128(xq.data_ptr(), ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(),
-                                   0 if bias is None else bias.data_ptr(), y.data_ptr(), n, _TYPE[out_dtype], m, n, k,
-                                   _stream(dev))
-    return y
-
-
 def linear(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None,
            out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``x @ weight.T (+ bias)``: ``x`` [..., k] is quantised (as ``quantize`` does) and multiplied in 8 bits with
@@ -203,7 +180,7 @@ def linear(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None,
         if isinstance(weight, torch.Tensor):
             return _Linear.apply(x, weight, bias, None)
         return _Linear.apply(x, None, bias, weight)
-    return _forward(x, weight, bias, out_dtype)[0]
+    return _forward(x, weight, bias, out_dtype, False)[0]
 
 
 def _weight_pair(weight):
@@ -213,12 +190,39 @@ def _weight_pair(weight):
     return _pair(quantize(weight) if isinstance(weight, torch.Tensor) else weight, "weight")
 
 
-def _forward(x, weight, bias, out_dtype):
-    wp = _weight_pair(weight)
-    if x.dim() == 0 or x.shape[-1] != wp[3]:
-        raise ValueError(f"x has shape {tuple(x.shape)}, the weight {wp[3]} columns")
-    xp = _pair(quantize(x), "x")
-    return _product(xp, wp, bias, out_dtype, x.shape[:-1]), xp, wp
+def _forward(x, weight, bias, out_dtype, keep: bool):
+    """(result, x's pair in two dimensions or None, the weight's pair)."""
+    wq, ws, n, k, ldw = wp = _weight_pair(weight)
+    if x.dim() == 0 or x.shape[-1] != k:
+        raise ValueError(f"x has shape {tuple(x.shape)}, the weight {k} columns")
+    lead = x.shape[:-1]
+    x, m, _, ldx = _matrix(x.detach(), "x")
+    dev = x.device
+    _same_device(dev, weight=wq, bias=bias)
+    if bias is not None:
+        if bias.shape != (n,):
+            raise ValueError(f"bias must have shape ({n},); got {tuple(bias.shape)}")
+        if bias.dtype != out_dtype:
+            raise ValueError(f"bias must be {out_dtype} like the result; got {bias.dtype}")
+        bias = bias.detach().contiguous()
+    y = torch.empty((*lead, n), dtype=out_dtype, device=dev)
+    if k == 0:
+        return (y.zero_() if bias is None else y.copy_(bias.expand_as(y))), quantize(x) if keep else None, wp
+    C = native()
+    work_bytes = C.linear_work_bytes(m, k)
+    if keep:
+        (q, scales), pitch = _empty_pair((m, k), dev)
+        work = torch.empty(work_bytes, dtype=torch.uint8, device=dev)
+        ptrs = q.data_ptr(), pitch, scales.data_ptr(), work.data_ptr()
+    else:
+        pitch = -(-k // 16) * 16
+        work = torch.empty(work_bytes + m * pitch, dtype=torch.uint8, device=dev)
+        ptrs = work.data_ptr() + work_bytes, pitch, 0, work.data_ptr()
+    with _on(dev):
+        C.k_linear_block128(x.data_ptr(), ldx, _TYPE[x.dtype], *ptrs, work_bytes, wq.data_ptr(), ldw, ws.data_ptr(),
+                            0 if bias is None else bias.data_ptr(), y.data_ptr(), n, _TYPE[out_dtype], m, n, k,
+                            _stream(dev))
+    return y, (q, scales) if keep else None, wp
 
 
 def _gradient(dy: torch.Tensor, other: Block128, what: str):
@@ -265,9 +269,9 @@ def linear_weight_grad(dy: torch.Tensor, x: Block128, out_dtype: torch.dtype = t
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, pair):
-        y, xp, wp = _forward(x, pair if weight is None else weight, bias, torch.bfloat16)
         need_dw = weight is not None and weight.requires_grad
-        ctx.save_for_backward(*(xp[:2] if need_dw else (None, None)),
+        y, xp, wp = _forward(x, pair if weight is None else weight, bias, torch.bfloat16, need_dw)
+        ctx.save_for_backward(*(xp if need_dw else (None, None)),
                               *(wp[:2] if x.requires_grad else (None, None)))
         ctx.x_shape = x.shape
         ctx.weight_dtype = None if weight is None else weight.dtype

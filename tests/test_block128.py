@@ -87,14 +87,16 @@ def test_quantize_launcher_refuses(args):
 
 @pytest.mark.parametrize("args", [
     dict(a=0), dict(q=0), dict(s=0), dict(o=0), dict(q=A + 4), dict(ldq=200), dict(lda=255), dict(ldo=1),
-    dict(m=-1), dict(n=1 << 40), dict(red=0)])
+    dict(m=-1), dict(n=1 << 40), dict(red=0), dict(w=0), dict(w=A + 8), dict(wb=100)])
 def test_product_launchers_refuse(args):
-    a = dict(a=A, lda=256, q=A, ldq=256, s=A, o=A, ldo=256, m=256, n=256, red=256) | args
+    a = dict(a=A, lda=256, q=A, ldq=256, s=A, o=A, ldo=256, m=256, n=256, red=256, w=A, wb=1 << 20) | args
     C = native()
     red = a["red"]
     with pytest.raises(RuntimeError, match="invalid argument"):  # red: the length that is summed over
-        C.k_matmul_block128(a["a"], a["lda"], a["s"], a["q"], a["ldq"], a["s"], 0, a["o"], a["ldo"], 0, a["m"], a["n"],
-                            red, 0)
+        C.k_linear_block128(a["a"], a["lda"], 0, a["a"], a["lda"], a["s"], a["w"], a["wb"], a["q"], a["ldq"], a["s"], 0,
+                            a["o"], a["ldo"], 0, a["m"], a["n"], red, 0)
+    if "w" in args or "wb" in args:
+        return
     with pytest.raises(RuntimeError, match="invalid argument"):
         C.k_matmul_input_grad(a["a"], a["lda"], a["q"], a["ldq"], a["s"], a["o"], a["ldo"], 0, a["m"], red, a["n"], 0)
     with pytest.raises(RuntimeError, match="invalid argument"):
@@ -105,7 +107,7 @@ def test_empty_shapes_launch_nothing():
     n = native().kernel_launch_count()
     native().k_quantize_block128(0, 128, 0, 0, 128, 0, 0, 128, 0)
     native().k_swiglu_forward(0, 8, 0, 8, 0, 0, 8, 0, 0, 0, 0, 16, 0, 8, 0)
-    native().k_matmul_block128(0, 128, 0, 0, 128, 0, 0, 0, 4, 0, 0, 4, 128, 0)
+    native().k_linear_block128(0, 128, 0, 0, 128, 0, 0, 0, 0, 128, 0, 0, 0, 4, 0, 0, 4, 128, 0)
     native().k_matmul_input_grad(0, 4, 0, 128, 0, 0, 128, 0, 0, 4, 128, 0)
     native().k_matmul_weight_grad(0, 4, 0, 128, 0, 0, 128, 0, 3, 0, 128, 0)
     assert native().kernel_launch_count() == n
