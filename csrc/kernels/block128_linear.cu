@@ -69,6 +69,14 @@ struct Config {
     static constexpr uint32_t smem = off_misc + 16 + 1024;  // + alignment of the base
     static constexpr int CPT = BN / (EW / 4);                  // columns of one epilogue thread
     static constexpr int CH = CPT % 32 ? 16 : 32;            // columns of one tensor-memory load
+    // The epilogue either reads all its columns of a product at once, which
+    // frees the buffer before the arithmetic, or two loads in turn where there
+    // are no registers for that. The first form of eight warps needs more
+    // registers than an even share: the four other warps give up theirs.
+    static constexpr bool ALL = EW == 8 || CPT <= 32;
+    static constexpr bool SHIFT = EW == 8;
+    static constexpr int kEven = 168, kFew = 40, kMany = 232;
+    static_assert(!SHIFT || 128 * kFew + 256 * kMany <= 384 * kEven, "a split that the block has registers for");
     static_assert(tmem_used <= 512 && tmem_cols * per_sm <= 512, "tensor memory");
     static_assert(smem * per_sm <= 227 * 1024, "shared memory");
     static_assert(CPT % CH == 0 && BN % 16 == 0 && (CG == 1 || BN % 32 == 0), "");
@@ -85,13 +93,34 @@ __device__ __forceinline__ float bias_at(const Args& a, uint32_t i) {
     return a.type == 0 ? as_float<__nv_bfloat16>(a.bias, i) : a.type == 1 ? as_float<__half>(a.bias, i)
                                                                         : as_float<float>(a.bias, i);
 }
+template <typename T>
+__device__ __forceinline__ T rounded(float v);
+template <>
+__device__ __forceinline__ __nv_bfloat16 rounded(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half rounded(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ float rounded(float v) { return v; }
+
 __device__ __forceinline__ void store_one(const Args& a, int64_t at, float v) {
     if (a.type == 0)
-        static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+        static_cast<__nv_bfloat16*>(a.out)[at] = rounded<__nv_bfloat16>(v);
     else if (a.type == 1)
-        static_cast<__half*>(a.out)[at] = __float2half_rn(v);
+        static_cast<__half*>(a.out)[at] = rounded<__half>(v);
     else
         static_cast<float*>(a.out)[at] = v;
+}
+// One lane's results: output `row` for tokens c0 and on.
+template <typename T, int N>
+__device__ __forceinline__ void store_column(const Args& a, uint32_t row, uint32_t c0, const uint64_t (&acc)[N / 2],
+                                             float add) {
+    T* p = static_cast<T*>(a.out) + int64_t(c0) * a.ld + row;
+    const uint32_t left = a.m > c0 ? a.m - c0 : 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i, p += a.ld) {
+        const float2 f = unpack2(acc[i / 2]);
+        if (uint32_t(i) < left) *p = rounded<T>((i & 1 ? f.y : f.x) + add);
+    }
 }
 
 template <typename C>
@@ -143,8 +172,9 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
         *tm = in / wide;
     };
 
-    if (warp == 0) {
-        if (lane == 0) {
+    if (warp < 4) {
+        if (C::SHIFT) regs_less<C::kFew>();
+        if (warp == 0 && lane == 0) {
             prefetch_map(&map_w);
             prefetch_map(&map_x);
             prefetch_map(&map_sx);
@@ -183,8 +213,7 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                     }
             }
         }
-    } else if (warp == 1) {
-        if (lane == 0 && half == 0) {
+        if (warp == 1 && lane == 0 && half == 0) {
             constexpr uint32_t idesc = instr_desc_mxf8(kLanes * C::CG, C::BN);
             uint32_t it = 0;
             bool ok = true;
@@ -208,7 +237,15 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                     mma_commit<C::CG>(tfull(b));
                 }
         }
-    } else if (warp >= 4) {
+        // Even shares of registers again, for the code that all warps run; not
+        // before every warp is done with its own.
+        __syncwarp();
+        if (C::SHIFT) {
+            __syncthreads();
+            regs_more<C::kEven>();
+        }
+    } else {
+        if (C::SHIFT) regs_more<C::kMany>();
         const uint32_t quad = warp % 4, mine = (warp - 4) / 4 * C::CPT;  // lanes, first column
         const uint32_t my_lane = quad * 32 + lane;
         uint32_t it = 0;
@@ -232,26 +269,44 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t from = tmem + b * C::BN + mine + (quad * 32 << 16);
-                uint32_t v[2][C::CH];
-                tmem_ld(from, v[0]);
-                tmem_ld_wait(v[0]);
-#pragma unroll
-                for (int c = 0; c < C::CPT / C::CH; ++c) {
-                    if (c + 1 < C::CPT / C::CH) tmem_ld(from + (c + 1) * C::CH, v[(c + 1) & 1]);
+                constexpr int NC = C::CPT / C::CH;
+                uint32_t v[C::ALL ? NC : 2][C::CH];
+                auto add = [&](int c) {
+                    uint32_t(&w)[C::CH] = v[C::ALL ? c : c & 1];
 #pragma unroll
                     for (int i = 0; i < C::CH; i += 2) {
                         uint64_t* d = acc + (c * C::CH + i) / 2;
-                        *d = fma2(pack2(v[c & 1][i], v[c & 1][i + 1]), s2, *d);
+                        *d = fma2(pack2(w[i], w[i + 1]), s2, *d);
                     }
-                    if (c + 1 < C::CPT / C::CH) tmem_ld_wait(v[(c + 1) & 1]);
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if (C::CG == 2)
-                        mbar_arrive_remote(map_to_rank(tempty(b), 0));
-                    else
-                        mbar_arrive(tempty(b));
+                };
+                auto release = [&] {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (C::CG == 2)
+                            mbar_arrive_remote(map_to_rank(tempty(b), 0));
+                        else
+                            mbar_arrive(tempty(b));
+                    }
+                };
+                if (C::ALL) {
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) tmem_ld(from + c * C::CH, v[C::ALL ? c : 0]);
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) tmem_ld_wait(v[C::ALL ? c : 0]);  // the first waits for all
+                    release();
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) add(c);
+                } else {
+                    tmem_ld(from, v[0]);
+                    tmem_ld_wait(v[0]);
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        if (c + 1 < NC) tmem_ld(from + (c + 1) * C::CH, v[C::ALL ? 0 : (c + 1) & 1]);
+                        add(c);
+                        if (c + 1 < NC) tmem_ld_wait(v[C::ALL ? 0 : (c + 1) & 1]);
+                    }
+                    release();
                 }
             }
             if (C::CG == 1 && a.split > 1) {
@@ -273,16 +328,21 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
             if (ok && row < a.n) {
                 const float add = a.bias ? bias_at(a, row) : 0.f;
                 const uint32_t c0 = tm * C::BN + mine;
-#pragma unroll
-                for (int i = 0; i < C::CPT; ++i) {
-                    const float2 f = unpack2(acc[i / 2]);
-                    if (c0 + i < a.m) store_one(a, int64_t(c0 + i) * a.ld + row, (i & 1 ? f.y : f.x) + add);
-                }
+                if (a.type == 0)
+                    store_column<__nv_bfloat16, C::CPT>(a, row, c0, acc, add);
+                else if (a.type == 1)
+                    store_column<__half, C::CPT>(a, row, c0, acc, add);
+                else
+                    store_column<float, C::CPT>(a, row, c0, acc, add);
             }
             __syncwarp();
         }
+        __syncwarp();
+        if (C::SHIFT) {
+            __syncthreads();
+            regs_less<C::kEven>();
+        }
     }
-    __syncwarp();
     if (C::CG == 1 && a.split > 1) {
         __syncthreads();
         cluster_sync();

@@ -44,7 +44,7 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -77,6 +77,7 @@ struct Guard {
 
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Guard& g, uint32_t code) {
+    if (CLUSTER ? mbar_test_cluster(bar, parity) : mbar_test(bar, parity)) return true;
     const long long t0 = clock64();
     while (!(CLUSTER ? mbar_test_cluster(bar, parity) : mbar_test(bar, parity))) {
         if (*g.abort) return false;
@@ -281,6 +282,17 @@ __host__ __device__ constexpr uint32_t instr_desc(int m, int n, uint32_t fmt, bo
 // The one of products with factors: e4m3 operands, e8m0 factors in byte 0.
 __host__ __device__ constexpr uint32_t instr_desc_mxf8(int m, int n) {
     return uint32_t(n >> 3) << 17 | 1u << 23 | uint32_t(m >> 4) << 24;
+}
+
+// A warpgroup's share of registers. Changes of one warpgroup need a barrier of
+// all its warps in between; an increase waits until the block has enough left.
+template <int N>
+__device__ __forceinline__ void regs_more() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_less() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // ---- packed fp32 pairs
