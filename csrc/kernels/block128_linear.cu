@@ -9,10 +9,10 @@
 // warps add sw P_b to fp32 registers while the next block's product runs.
 //
 // The rows of w lie on the 128 lanes of tensor memory, so that sw is one
-// register of each epilogue thread and the addition one packed multiply-add
-// for two results; the tokens lie on its BN columns. With few tokens the tile
+// register of each epilogue thread and the addition one multiply-add for a
+// result; the tokens lie on its BN columns. With few tokens the tile
 // then holds little but weights. Per 128 x BN tile and block the tensor core
-// takes 2 BN cycles and the epilogue's multiply-adds BN.
+// takes 2 BN cycles and the epilogue's multiply-adds BN issue slots of each scheduler.
 //
 // Warps: 0 loads (TMA in the 128-byte swizzle), 1 issues the products, 2 owns
 // the tensor memory, 3 idles, the rest are the epilogue.
@@ -112,15 +112,12 @@ __device__ __forceinline__ void store_one(const Args& a, int64_t at, float v) {
 }
 // One lane's results: output `row` for tokens c0 and on.
 template <typename T, int N>
-__device__ __forceinline__ void store_column(const Args& a, uint32_t row, uint32_t c0, const uint64_t (&acc)[N / 2],
-                                             float add) {
+__device__ __forceinline__ void store_column(const Args& a, uint32_t row, uint32_t c0, const float (&acc)[N], float add) {
     T* p = static_cast<T*>(a.out) + int64_t(c0) * a.ld + row;
     const uint32_t left = a.m > c0 ? a.m - c0 : 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i, p += a.ld) {
-        const float2 f = unpack2(acc[i / 2]);
-        if (uint32_t(i) < left) *p = rounded<T>((i & 1 ? f.y : f.x) + add);
-    }
+    for (int i = 0; i < N; ++i, p += a.ld)
+        if (uint32_t(i) < left) *p = rounded<T>(acc[i] + add);
 }
 
 template <typename C>
@@ -138,7 +135,8 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
     volatile uint32_t* const misc = reinterpret_cast<volatile uint32_t*>(sm + C::off_misc);  // tensor memory, abort
     const Guard guard{misc + 1, a.error};
 
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    // one value for a warp, so that what the issuing warps compute stays in uniform registers
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const uint32_t in_cluster = C::CG == 2 || a.split > 1 ? cluster_rank() : 0;
     const uint32_t half = C::CG == 2 ? in_cluster : 0;  // which CTA of the pair
     const uint32_t part = C::CG == 1 ? in_cluster : 0;  // which part of the sum
@@ -174,67 +172,80 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
 
     if (warp < 4) {
         if (C::SHIFT) regs_less<C::kFew>();
-        if (warp == 0 && lane == 0) {
-            prefetch_map(&map_w);
-            prefetch_map(&map_x);
-            prefetch_map(&map_sx);
-            uint32_t it = 0;
+        if (warp == 0) {
+            const bool leader = elect_one();
+            if (leader) {
+                prefetch_map(&map_w);
+                prefetch_map(&map_x);
+                prefetch_map(&map_sx);
+            }
+            uint32_t it = 0, s = 0, phase = 1;
             bool ok = true;
             for (uint32_t t = first_tile; ok && t < tiles; t += step) {
                 uint32_t n0, tm;
                 place(t, &n0, &tm);
                 for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                    const uint32_t s = it % C::ST;
-                    if (!(ok = mbar_wait(empty(s), (it / C::ST & 1) ^ 1, guard, kWaitEmpty))) break;
-                    const uint32_t dst = base + s * C::stage_pitch;
-                    const uint32_t dst_sx = dst + C::w_bytes + C::x_bytes;
-                    if (C::CG == 1) {
-                        mbar_expect(full(s), C::stage_bytes);
-                        tma_load(dst, &map_w, kb * kBlock, n0, full(s));
-                        tma_load(dst + C::w_bytes, &map_x, kb * kBlock, tm * C::BN, full(s));
-                        tma_load(dst_sx, &map_sx, 0, tm * a.nb + kb, full(s));
-                    } else {
-                        // The tiles of both CTAs count on the first one's
-                        // barrier, where the products wait. Both need all of
-                        // the factors, which go from each CTA's own shared
-                        // memory to its own tensor memory.
-                        if (half == 0) mbar_expect(full(s), 2 * C::stage_bytes);
-                        const uint32_t b = map_to_rank(full(s), 0);
-                        tma_load_pair(dst, &map_w, kb * kBlock, n0, b);
-                        tma_load_pair(dst + C::w_bytes, &map_x, kb * kBlock, tm * C::BN + half * (C::BN / 2), b);
-                        tma_load_pair(dst_sx, &map_sx, 0, tm * a.nb + kb, b);
+                    ok = __all_sync(0xffffffffu, mbar_wait(empty(s), phase, guard, kWaitEmpty));
+                    if (!ok) break;
+                    if (leader) {
+                        const uint32_t dst = base + s * C::stage_pitch, dst_sx = dst + C::w_bytes + C::x_bytes;
+                        if (C::CG == 1) {
+                            mbar_expect(full(s), C::stage_bytes);
+                            tma_load(dst, &map_w, kb * kBlock, n0, full(s));
+                            tma_load(dst + C::w_bytes, &map_x, kb * kBlock, tm * C::BN, full(s));
+                            tma_load(dst_sx, &map_sx, 0, tm * a.nb + kb, full(s));
+                        } else {
+                            // The tiles of both CTAs count on the first one's
+                            // barrier, where the products wait. Both need all
+                            // of the factors, which go from each CTA's own
+                            // shared memory to its own tensor memory.
+                            if (half == 0) mbar_expect(full(s), 2 * C::stage_bytes);
+                            const uint32_t b = map_to_rank(full(s), 0);
+                            tma_load_pair(dst, &map_w, kb * kBlock, n0, b);
+                            tma_load_pair(dst + C::w_bytes, &map_x, kb * kBlock, tm * C::BN + half * (C::BN / 2), b);
+                            tma_load_pair(dst_sx, &map_sx, 0, tm * a.nb + kb, b);
+                        }
                     }
+                    __syncwarp();
+                    if (++s == C::ST) s = 0, phase ^= 1;
                 }
             }
-            if (*guard.abort && half == 0) {  // let copies in flight land before the block retires
+            if (*guard.abort && half == 0 && leader) {  // let copies in flight land before the block retires
                 const long long t0 = clock64();
                 for (uint32_t i = it > C::ST ? it - C::ST : 0; i < it; ++i)
                     while (!mbar_test(full(i % C::ST), i / C::ST & 1) && clock64() - t0 < kWaitCycles / 8) {
                     }
             }
+            __syncwarp();
         }
-        if (warp == 1 && lane == 0 && half == 0) {
+        if (warp == 1 && half == 0) {
             constexpr uint32_t idesc = instr_desc_mxf8(kLanes * C::CG, C::BN);
-            uint32_t it = 0;
+            const bool leader = elect_one();
+            uint32_t it = 0, s = 0, b = 0, sphase = 0, bphase = 1;
             bool ok = true;
             for (uint32_t t = first_tile; ok && t < tiles; t += step)
                 for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                    const uint32_t s = it % C::ST, b = it % C::NBUF;
-                    ok = mbar_wait<C::CG == 2>(tempty(b), (it / C::NBUF & 1) ^ 1, guard, kWaitTmemEmpty) &&
-                         mbar_wait(full(s), it / C::ST & 1, guard, kWaitFull);
+                    ok = mbar_wait<C::CG == 2>(tempty(b), bphase, guard, kWaitTmemEmpty) &&
+                         mbar_wait(full(s), sphase, guard, kWaitFull);
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t src = base + s * C::stage_pitch;
+                    if (leader) {
+                        const uint32_t src = base + s * C::stage_pitch, d = tmem + b * C::BN;
 #pragma unroll
-                    for (uint32_t i = 0; i < C::sx_words; i += 128)
-                        scales_to_tmem<C::CG>(tmem + C::tmem_sx + i / 32, src + C::w_bytes + C::x_bytes + i * 4);
-                    const uint64_t dw = operand_desc(src), dx = operand_desc(src + C::w_bytes);
+                        for (uint32_t i = 0; i < C::sx_words; i += 128)
+                            scales_to_tmem<C::CG>(tmem + C::tmem_sx + i / 32, src + C::w_bytes + C::x_bytes + i * 4);
+                        const uint64_t dw = operand_desc(src), dx = operand_desc(src + C::w_bytes);
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k)  // 32 values, 32 bytes, a step
-                        mma_mxf8<C::CG>(tmem + b * C::BN, dw + 2 * k, dx + 2 * k, idesc, tmem + C::tmem_sw,
-                                        tmem + C::tmem_sx, k > 0);
-                    mma_commit<C::CG>(empty(s));
-                    mma_commit<C::CG>(tfull(b));
+                        for (uint32_t k = 0; k < 4; ++k)  // 32 values, 32 bytes, a step
+                            mma_mxf8<C::CG>(d, dw + 2 * k, dx + 2 * k, idesc, tmem + C::tmem_sw, tmem + C::tmem_sx,
+                                            k > 0);
+                        mma_commit<C::CG>(empty(s));
+                        mma_commit<C::CG>(tfull(b));
+                    }
+                    __syncwarp();
+                    if (++s == C::ST) s = 0, sphase ^= 1;
+                    if (++b == C::NBUF) b = 0, bphase ^= 1;
                 }
         }
         // Even shares of registers again, for the code that all warps run; not
@@ -256,12 +267,12 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
             const uint32_t row = n0 + my_lane;
             const float* sw = a.scale_w + uint64_t(min(row, a.n - 1)) * a.nb;
             float next = __ldg(sw + kb0);
-            uint64_t acc[C::CPT / 2];
+            float acc[C::CPT];
 #pragma unroll
-            for (int i = 0; i < C::CPT / 2; ++i) acc[i] = 0;
+            for (int i = 0; i < C::CPT; ++i) acc[i] = 0.f;
             for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
                 const uint32_t b = it % C::NBUF;
-                const uint64_t s2 = pack2(__float_as_uint(next), __float_as_uint(next));
+                const float scale = next;
                 if (kb + 1 < kb1) next = __ldg(sw + kb + 1);
                 ok = mbar_wait(tfull(b), it / C::NBUF & 1, guard, kWaitTmemFull);
                 ok = __all_sync(0xffffffffu, ok);
@@ -274,10 +285,7 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                 auto add = [&](int c) {
                     uint32_t(&w)[C::CH] = v[C::ALL ? c : c & 1];
 #pragma unroll
-                    for (int i = 0; i < C::CH; i += 2) {
-                        uint64_t* d = acc + (c * C::CH + i) / 2;
-                        *d = fma2(pack2(w[i], w[i + 1]), s2, *d);
-                    }
+                    for (int i = 0; i < C::CH; ++i) add_scaled(acc[c * C::CH + i], w[i], scale);
                 };
                 auto release = [&] {
                     tc_fence_before();
@@ -292,19 +300,18 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                 if (C::ALL) {
 #pragma unroll
                     for (int c = 0; c < NC; ++c) tmem_ld(from + c * C::CH, v[C::ALL ? c : 0]);
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) tmem_ld_wait(v[C::ALL ? c : 0]);  // the first waits for all
+                    tmem_ld_wait();
                     release();
 #pragma unroll
                     for (int c = 0; c < NC; ++c) add(c);
                 } else {
                     tmem_ld(from, v[0]);
-                    tmem_ld_wait(v[0]);
+                    tmem_ld_wait();
 #pragma unroll
                     for (int c = 0; c < NC; ++c) {
                         if (c + 1 < NC) tmem_ld(from + (c + 1) * C::CH, v[C::ALL ? 0 : (c + 1) & 1]);
                         add(c);
-                        if (c + 1 < NC) tmem_ld_wait(v[C::ALL ? 0 : (c + 1) & 1]);
+                        if (c + 1 < NC) tmem_ld_wait();
                     }
                     release();
                 }
@@ -316,11 +323,7 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                 // the columns, in the order of the parts.
                 float* part_sum = reinterpret_cast<float*>(sm);
 #pragma unroll
-                for (int i = 0; i < C::CPT / 2; ++i) {
-                    const float2 f = unpack2(acc[i]);
-                    part_sum[(2 * i) * kLanes + my_lane] = f.x;
-                    part_sum[(2 * i + 1) * kLanes + my_lane] = f.y;
-                }
+                for (int i = 0; i < C::CPT; ++i) part_sum[i * kLanes + my_lane] = acc[i];
                 break;
             }
             // The lanes past the last row take no other way through the loop:

@@ -234,7 +234,6 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 }
 
 #define OFLD_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
-#define OFLD_W4(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
 
 // 16 / 32 consecutive columns of this warp's 32 lanes (one lane a thread).
 __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&v)[16]) {
@@ -251,19 +250,15 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&v)[32]) {
           OFLD_R4(v, 28)
         : "r"(addr));
 }
-// Waits for this thread's loads; the registers go through it so that no use
-// of them moves ahead of the wait.
-__device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : OFLD_W4(v, 0), OFLD_W4(v, 4), OFLD_W4(v, 8), OFLD_W4(v, 12)::"memory");
-}
-__device__ __forceinline__ void tmem_ld_wait(uint32_t (&v)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : OFLD_W4(v, 0), OFLD_W4(v, 4), OFLD_W4(v, 8), OFLD_W4(v, 12), OFLD_W4(v, 16), OFLD_W4(v, 20),
-                   OFLD_W4(v, 24), OFLD_W4(v, 28)::"memory");
+// Waits for this thread's loads. What uses their registers is volatile too
+// (add_scaled), so that the compiler moves none of it ahead of the wait.
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// acc += v * scale. Not as packed pairs: the compiler moves the loaded
+// registers into pairs of their own, which costs more than the pairs save.
+__device__ __forceinline__ void add_scaled(float& acc, uint32_t v, float scale) {
+    asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc) : "f"(__uint_as_float(v)), "f"(scale));
 }
 #undef OFLD_R4
-#undef OFLD_W4
 
 // Shared-memory operand in the 128-byte swizzle: rows of 128 bytes, groups of
 // eight rows 1024 bytes apart. K-major: a row is 128 bytes of the summed
@@ -293,29 +288,6 @@ __device__ __forceinline__ void regs_more() {
 template <int N>
 __device__ __forceinline__ void regs_less() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-// ---- packed fp32 pairs
-
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-    uint32_t lo, hi;
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
-    return make_float2(__uint_as_float(lo), __uint_as_float(hi));
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
 }
 
 }  // namespace sm100
