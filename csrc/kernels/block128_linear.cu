@@ -225,16 +225,22 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
             bool ok = true;
             for (uint32_t t = first_tile; ok && t < tiles; t += step)
                 for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                    ok = mbar_wait<C::CG == 2>(tempty(b), bphase, guard, kWaitTmemEmpty) &&
-                         mbar_wait(full(s), sphase, guard, kWaitFull);
-                    ok = __all_sync(0xffffffffu, ok);
+                    // the factors go ahead of the wait for a buffer: copies and products run in order
+                    const uint32_t src = base + s * C::stage_pitch;
+                    ok = __all_sync(0xffffffffu, mbar_wait(full(s), sphase, guard, kWaitFull));
                     if (!ok) break;
                     tc_fence_after();
                     if (leader) {
-                        const uint32_t src = base + s * C::stage_pitch, d = tmem + b * C::BN;
 #pragma unroll
                         for (uint32_t i = 0; i < C::sx_words; i += 128)
                             scales_to_tmem<C::CG>(tmem + C::tmem_sx + i / 32, src + C::w_bytes + C::x_bytes + i * 4);
+                    }
+                    __syncwarp();
+                    ok = __all_sync(0xffffffffu, mbar_wait<C::CG == 2>(tempty(b), bphase, guard, kWaitTmemEmpty));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (leader) {
+                        const uint32_t d = tmem + b * C::BN;
                         const uint64_t dw = operand_desc(src), dx = operand_desc(src + C::w_bytes);
 #pragma unroll
                         for (uint32_t k = 0; k < 4; ++k)  // 32 values, 32 bytes, a step

@@ -43,8 +43,15 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// For an order of events alone (tensor memory has been read): writes to memory
+// are not covered.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The same for memory that this thread has written: visible to what the other
+// CTA does after its wait.
+__device__ __forceinline__ void mbar_release_remote(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -110,6 +117,15 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
         "l"(m), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
+// Four bytes, zeros when !valid.
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+// Arrives once all earlier cp.async of this thread have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+// Makes this thread's writes to shared memory visible to copies and products.
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ---- clusters
@@ -233,6 +249,7 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
             : "memory");
 }
 
+#define OFLD_W4(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
 #define OFLD_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
 
 // 16 / 32 consecutive columns of this warp's 32 lanes (one lane a thread).
@@ -253,12 +270,20 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&v)[32]) {
 // Waits for this thread's loads. What uses their registers is volatile too
 // (add_scaled), so that the compiler moves none of it ahead of the wait.
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// The same for loads whose registers go into ordinary code: they pass through
+// the wait.
+__device__ __forceinline__ void tmem_ld_keep(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : OFLD_W4(v, 0), OFLD_W4(v, 4), OFLD_W4(v, 8), OFLD_W4(v, 12), OFLD_W4(v, 16), OFLD_W4(v, 20),
+                   OFLD_W4(v, 24), OFLD_W4(v, 28)::"memory");
+}
 // acc += v * scale. Not as packed pairs: the compiler moves the loaded
 // registers into pairs of their own, which costs more than the pairs save.
 __device__ __forceinline__ void add_scaled(float& acc, uint32_t v, float scale) {
     asm volatile("fma.rn.f32 %0, %1, %2, %0;" : "+f"(acc) : "f"(__uint_as_float(v)), "f"(scale));
 }
 #undef OFLD_R4
+#undef OFLD_W4
 
 // Shared-memory operand in the 128-byte swizzle: rows of 128 bytes, groups of
 // eight rows 1024 bytes apart. K-major: a row is 128 bytes of the summed

@@ -36,7 +36,7 @@ DAEMON = ["daemon/config.cpp", "daemon/daemon.cpp", "daemon/slots.cpp", "daemon/
           "daemon/nvme.cpp", "daemon/canonical.cpp", "daemon/rollout.cpp", "daemon/persist.cpp"]
 AGENT = ["agent/agent.cpp"]
 KERNELS = ["kernels/offload_kernels.cu", "kernels/weight_sync.cu", "kernels/hash_noalloc.cu",
-           "kernels/block128.cu", "kernels/block128_linear.cu", "kernels/block128_matmul.cu"]
+           "kernels/block128.cu", "kernels/block128_linear.cu", "kernels/block128_grad.cu"]
 KERNEL_HOST = ["kernels/timing.cpp", "kernels/block128_host.cpp"]
 FABRIC = ["fabric/fabric.cpp", "fabric/vmm.cpp"]
 MODULE = ["python/module.cpp", "python/fabric_bind.cpp", "python/block128_bind.cpp"]
