@@ -40,9 +40,10 @@ using namespace sm100;
 
 constexpr uint32_t kSide = 128;  // rows of A and columns of Q of one CTA
 constexpr uint32_t kStep = 64;   // of t
-constexpr uint32_t kConverters = 8, kThreads = 512;
+constexpr uint32_t kGroups = 2, kGroupWarps = 4;  // of converters: a group takes every second step
+constexpr uint32_t kThreads = 512;
 
-enum : uint32_t { kWaitEmpty = 201, kWaitFull, kWaitScales, kWaitConverted, kWaitTmemEmpty, kWaitTmemFull };
+enum : uint32_t { kWaitEmpty = 201, kWaitFull, kWaitConverted, kWaitTmemEmpty, kWaitTmemFull };
 
 struct Args {
     const float* scales;
@@ -65,7 +66,7 @@ struct Config {
     static constexpr uint32_t off_q = a_bytes, off_b = off_q + q_bytes, stage = off_b + b_bytes;
     static constexpr uint32_t off_scale = ST * stage;
     static constexpr uint32_t off_bar = off_scale + ST * kStep * 4;
-    static constexpr uint32_t off_misc = off_bar + (4 * ST + 4) * 8;
+    static constexpr uint32_t off_misc = off_bar + (3 * ST + 4) * 8;
     static constexpr uint32_t smem = off_misc + 16 + 1024;
     static constexpr uint32_t tmem_cols = 2 * BN;
     static_assert(smem <= 227 * 1024 && tmem_cols <= 512, "");
@@ -131,12 +132,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
     uint8_t* const sm = raw + (base - smem_addr(raw));
     const uint32_t bar = base + C::off_bar;
-    auto full = [&](uint32_t s) { return bar + 8 * s; };                      // A and Q have landed in this CTA
-    auto scaled = [&](uint32_t s) { return bar + 8 * (C::ST + s); };          // the scales too
-    auto ready = [&](uint32_t s) { return bar + 8 * (2 * C::ST + s); };       // converted, in every CTA of the tile
-    auto empty = [&](uint32_t s) { return bar + 8 * (3 * C::ST + s); };       // multiplied
-    auto tfull = [&](uint32_t b) { return bar + 8 * (4 * C::ST + b); };
-    auto tempty = [&](uint32_t b) { return bar + 8 * (4 * C::ST + 2 + b); };
+    auto full = [&](uint32_t s) { return bar + 8 * s; };                 // A, Q and the scales have landed
+    auto ready = [&](uint32_t s) { return bar + 8 * (C::ST + s); };      // converted, in every CTA of the tile
+    auto empty = [&](uint32_t s) { return bar + 8 * (2 * C::ST + s); };  // multiplied
+    auto tfull = [&](uint32_t b) { return bar + 8 * (3 * C::ST + b); };
+    auto tempty = [&](uint32_t b) { return bar + 8 * (3 * C::ST + 2 + b); };
     volatile uint32_t* const misc = reinterpret_cast<volatile uint32_t*>(sm + C::off_misc);  // tensor memory, abort
     const Guard guard{misc + 1, a.error};
 
@@ -151,9 +151,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < C::ST; ++s) {
-            mbar_init(full(s), 1);
-            mbar_init(scaled(s), 32);
-            mbar_init(ready(s), kConverters * C::CG);
+            mbar_init(full(s), 1 + 32);  // the loads' thread, and each lane that fetches scales
+            mbar_init(ready(s), kGroupWarps * C::CG);
             mbar_init(empty(s), 1);
         }
         for (uint32_t b = 0; b < 2; ++b) mbar_init(tfull(b), 1), mbar_init(tempty(b), 4 * C::CG);
@@ -261,46 +260,56 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const bool valid = r < a.nt && jb < a.nb;
                     cp_async4(dst + (i + lane) * 4, valid ? a.scales + uint64_t(r) * a.nb + jb : a.scales, valid);
                 }
-                cp_async_arrive(scaled(s));
+                cp_async_arrive(full(s));
                 if (++s == C::ST) s = 0, phase ^= 1;
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp >= 8) {
-        const uint32_t id = threadIdx.x - 256, row = id / 4, quarter = id % 4, swz = row % 8;
-        uint32_t s = 0, phase = 0;
+        const uint32_t mine = (warp - 8) / kGroupWarps, id = threadIdx.x % (kGroupWarps * 32);
+        const uint32_t row = id / 2, h = id % 2, swz = row % 8;
+        uint32_t s = 0, phase = 0, turn = 0;
         bool ok = true;
         for (uint32_t t = first_tile; ok && t < tiles; t += step) {
             for (uint32_t k = t0; k < t1; ++k) {
-                ok = mbar_wait(scaled(s), phase, guard, kWaitScales) && mbar_wait(full(s), phase, guard, kWaitFull);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                const uint8_t* q = sm + s * C::stage + C::off_q + row * 128;
-                uint8_t* d = sm + s * C::stage + C::off_b + row * 128;
-                const float f = reinterpret_cast<const float*>(sm + C::off_scale)[s * kStep + row];
-                // 16 columns of each half of the tile: chunks of 16 bytes, at
-                // their place in the 128-byte swizzle of the source and of the
-                // two 64-column operand blocks
-                uint4 w[2];
+                if (turn == mine) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(full(s), phase, guard, kWaitFull));
+                    if (!ok) break;
+                    // Half a row: 64 columns, four chunks of 16 bytes of Q that
+                    // become eight of the operand, each at its place in the
+                    // 128-byte swizzle. The two halves take the chunks in
+                    // different order, which keeps eight lanes on eight banks.
+                    const uint8_t* q = sm + s * C::stage + C::off_q + row * 128;
+                    uint8_t* d = sm + s * C::stage + C::off_b + h * (C::b_bytes / 2) + row * 128;
+                    const float f = reinterpret_cast<const float*>(sm + C::off_scale)[s * kStep + row];
+                    uint4 w[4];
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h)
-                    w[h] = *reinterpret_cast<const uint4*>(q + (((quarter + 4 * h) ^ swz) * 16));
+                    for (uint32_t i = 0; i < 4; ++i)
+                        w[i] = *reinterpret_cast<const uint4*>(q + (((i ^ 2 * h) + 4 * h) ^ swz) * 16);
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    const uint2 c0 = convert4(w[h].x, f), c1 = convert4(w[h].y, f);
-                    const uint2 c2 = convert4(w[h].z, f), c3 = convert4(w[h].w, f);
-                    uint8_t* o = d + h * (C::b_bytes / 2);
-                    *reinterpret_cast<uint4*>(o + ((2 * quarter) ^ swz) * 16) = make_uint4(c0.x, c0.y, c1.x, c1.y);
-                    *reinterpret_cast<uint4*>(o + ((2 * quarter + 1) ^ swz) * 16) = make_uint4(c2.x, c2.y, c3.x, c3.y);
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const uint32_t c = 2 * (i ^ 2 * h);
+                        const uint2 c0 = convert4(w[i].x, f), c1 = convert4(w[i].y, f);
+                        const uint2 c2 = convert4(w[i].z, f), c3 = convert4(w[i].w, f);
+                        *reinterpret_cast<uint4*>(d + (c ^ swz) * 16) = make_uint4(c0.x, c0.y, c1.x, c1.y);
+                        *reinterpret_cast<uint4*>(d + ((c + 1) ^ swz) * 16) = make_uint4(c2.x, c2.y, c3.x, c3.y);
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    // The tensor core of this SM reads what was written here,
+                    // from this SM's shared memory: the fence above has put it
+                    // there, and the arrival at the first CTA of a pair, where
+                    // the product is issued, only has to come after it. A
+                    // release to the cluster would also wait for this SM's
+                    // global memory, 1300 to 1900 cycles a step.
+                    if (lane == 0) {
+                        if (C::CG == 2)
+                            mbar_arrive_remote(map_to_rank(ready(s), 0));
+                        else
+                            mbar_arrive(ready(s));
+                    }
                 }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    if (C::CG == 2)
-                        mbar_release_remote(map_to_rank(ready(s), 0));
-                    else
-                        mbar_arrive(ready(s));
-                }
+                turn = turn + 1 == kGroups ? 0 : turn + 1;
                 if (++s == C::ST) s = 0, phase ^= 1;
             }
         }
