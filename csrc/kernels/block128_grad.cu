@@ -17,9 +17,9 @@
 // tensor core spends 512 cycles on the step before. Few outputs: one CTA owns
 // 128 x 128, and the sum is split over a cluster of up to 8.
 //
-// Warps: 0 loads, 1 issues the products, 2 fetches the scales, 3 owns the
-// tensor memory, 4-7 store the results (of the last tile, while the next one's
-// sum runs in the other half of tensor memory), 8-15 convert.
+// Warps: 0 loads A, 1 issues the products, 2 loads Q and its scales, 3 owns
+// the tensor memory, 4-7 store the results (of the last tile, while the next
+// one's sum runs in the other half of tensor memory), 8-15 convert.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -43,7 +43,7 @@ constexpr uint32_t kStep = 64;   // of t
 constexpr uint32_t kGroups = 2, kGroupWarps = 4;  // of converters: a group takes every second step
 constexpr uint32_t kThreads = 512;
 
-enum : uint32_t { kWaitEmpty = 201, kWaitFull, kWaitConverted, kWaitTmemEmpty, kWaitTmemFull };
+enum : uint32_t { kWaitAEmpty = 201, kWaitQEmpty, kWaitBEmpty, kWaitAFull, kWaitQFull, kWaitBFull, kWaitTmemEmpty, kWaitTmemFull };
 
 struct Args {
     const float* scales;
@@ -52,7 +52,7 @@ struct Args {
     uint32_t ni, nj, nt, nb;
     uint32_t tiles_i, tiles_j, split;
     int type;  // FloatType
-    bool vec;  // 16-byte stores are aligned
+    bool tiled;  // the output can be stored in tiles (16-byte rows)
     uint32_t* error;
 };
 
@@ -60,18 +60,32 @@ struct Args {
 template <bool A_T_, int CG_>
 struct Config {
     static constexpr bool A_T = A_T_;
-    static constexpr int CG = CG_, ST = 5;
+    static constexpr int CG = CG_;
     static constexpr uint32_t BN = kSide * CG;
     static constexpr uint32_t a_bytes = kSide * kStep * 2, q_bytes = kSide * kStep, b_bytes = kSide * kStep * 2;
-    static constexpr uint32_t off_q = a_bytes, off_b = off_q + q_bytes, stage = off_b + b_bytes;
-    static constexpr uint32_t off_scale = ST * stage;
-    static constexpr uint32_t off_bar = off_scale + ST * kStep * 4;
-    static constexpr uint32_t off_misc = off_bar + (3 * ST + 4) * 8;
+    // Tiles in flight. From its load to the end of its product a tile of A
+    // lives about 3700 cycles, one of Q (until it is converted) 2500, a
+    // converted one 2000; a step takes 512.
+    static constexpr uint32_t NA = 7, NQ = 5, NB = 4;
+    static constexpr uint32_t off_q = NA * a_bytes, off_b = off_q + NQ * q_bytes, off_out = off_b + NB * b_bytes;
+    static constexpr uint32_t out_bytes = 32 * 64;  // of one storing warp: 32 rows of 64 bytes
+    static constexpr uint32_t off_scale = off_out + 4 * out_bytes;
+    static constexpr uint32_t off_bar = off_scale + NQ * kStep * 4;
+    static constexpr uint32_t off_misc = off_bar + (2 * (NA + NQ + NB) + 4) * 8;
     static constexpr uint32_t smem = off_misc + 16 + 1024;
     static constexpr uint32_t tmem_cols = 2 * BN;
     static_assert(smem <= 227 * 1024 && tmem_cols <= 512, "");
-    static_assert(a_bytes % 1024 == 0 && q_bytes % 1024 == 0 && b_bytes % 1024 == 0, "");
-    static_assert(ST * stage >= kSide * BN * 4 || CG == 2, "the split reduction's tile");
+    static_assert(a_bytes % 1024 == 0 && q_bytes % 1024 == 0 && b_bytes % 1024 == 0 && out_bytes % 1024 == 0, "");
+    static_assert(off_out >= kSide * BN * 4 || CG == 2, "the split reduction's tile");
+};
+
+// Position in a ring of N.
+template <uint32_t N>
+struct Ring {
+    uint32_t at = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++at == N) at = 0, phase ^= 1;
+    }
 };
 
 __device__ __forceinline__ uint32_t pack16(int type, float lo, float hi) {
@@ -90,33 +104,6 @@ __device__ __forceinline__ void store_one(const Args& a, int64_t at, float v) {
     else
         static_cast<float*>(a.out)[at] = v;
 }
-// Results of one row from column j on.
-template <int N>
-__device__ __forceinline__ void store_row(const Args& a, uint32_t row, uint32_t j, const uint32_t (&v)[N]) {
-    const int64_t at = int64_t(row) * a.ld + j;
-    if (a.vec && j + N <= a.nj) {
-        if (a.type == 2) {
-            uint4* p = reinterpret_cast<uint4*>(static_cast<float*>(a.out) + at);
-#pragma unroll
-            for (int i = 0; i < N; i += 4) p[i / 4] = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        } else {
-            uint4* p = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at);
-#pragma unroll
-            for (int i = 0; i < N; i += 8) {
-                uint32_t w[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    w[k] = pack16(a.type, __uint_as_float(v[i + 2 * k]), __uint_as_float(v[i + 2 * k + 1]));
-                p[i / 8] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (j + i < a.nj) store_one(a, at + i, __uint_as_float(v[i]));
-    }
-}
-
 // Four e4m3 values times a scale, as bf16.
 __device__ __forceinline__ uint2 convert4(uint32_t w, float s) {
     const __half2 lo(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w & 0xffff), __NV_E4M3));
@@ -127,16 +114,20 @@ __device__ __forceinline__ uint2 convert4(uint32_t w, float s) {
 
 template <typename C>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_grad(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_q, const Args a) {
+    k_grad(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_q,
+           const __grid_constant__ CUtensorMap map_out, const Args a) {
     extern __shared__ uint8_t raw[];
     const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
     uint8_t* const sm = raw + (base - smem_addr(raw));
     const uint32_t bar = base + C::off_bar;
-    auto full = [&](uint32_t s) { return bar + 8 * s; };                 // A, Q and the scales have landed
-    auto ready = [&](uint32_t s) { return bar + 8 * (C::ST + s); };      // converted, in every CTA of the tile
-    auto empty = [&](uint32_t s) { return bar + 8 * (2 * C::ST + s); };  // multiplied
-    auto tfull = [&](uint32_t b) { return bar + 8 * (3 * C::ST + b); };
-    auto tempty = [&](uint32_t b) { return bar + 8 * (3 * C::ST + 2 + b); };
+    auto a_full = [&](uint32_t s) { return bar + 8 * s; };  // in a pair: both CTAs' tiles, on the first one's barrier
+    auto a_empty = [&](uint32_t s) { return bar + 8 * (C::NA + s); };
+    auto q_full = [&](uint32_t s) { return bar + 8 * (2 * C::NA + s); };  // with its scales
+    auto q_empty = [&](uint32_t s) { return bar + 8 * (2 * C::NA + C::NQ + s); };
+    auto b_full = [&](uint32_t s) { return bar + 8 * (2 * (C::NA + C::NQ) + s); };  // converted, in every CTA of the tile
+    auto b_empty = [&](uint32_t s) { return bar + 8 * (2 * (C::NA + C::NQ) + C::NB + s); };
+    auto tfull = [&](uint32_t b) { return bar + 8 * (2 * (C::NA + C::NQ + C::NB) + b); };
+    auto tempty = [&](uint32_t b) { return bar + 8 * (2 * (C::NA + C::NQ + C::NB) + 2 + b); };
     volatile uint32_t* const misc = reinterpret_cast<volatile uint32_t*>(sm + C::off_misc);  // tensor memory, abort
     const Guard guard{misc + 1, a.error};
 
@@ -150,11 +141,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t0 = uint32_t(uint64_t(steps) * part / a.split), t1 = uint32_t(uint64_t(steps) * (part + 1) / a.split);
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < C::ST; ++s) {
-            mbar_init(full(s), 1 + 32);  // the loads' thread, and each lane that fetches scales
-            mbar_init(ready(s), kGroupWarps * C::CG);
-            mbar_init(empty(s), 1);
-        }
+        for (uint32_t s = 0; s < C::NA; ++s) mbar_init(a_full(s), 1), mbar_init(a_empty(s), 1);
+        // the load's thread, and each lane that fetches scales
+        for (uint32_t s = 0; s < C::NQ; ++s) mbar_init(q_full(s), 1 + 32), mbar_init(q_empty(s), kGroupWarps);
+        for (uint32_t s = 0; s < C::NB; ++s) mbar_init(b_full(s), kGroupWarps * C::CG), mbar_init(b_empty(s), 1);
         for (uint32_t b = 0; b < 2; ++b) mbar_init(tfull(b), 1), mbar_init(tempty(b), 4 * C::CG);
         mbar_init_fence();
         misc[1] = 0;
@@ -177,37 +167,40 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0) {
         const bool leader = elect_one();
-        if (leader) {
-            prefetch_map(&map_a);
-            prefetch_map(&map_q);
-        }
-        uint32_t it = 0, s = 0, phase = 1;
+        if (leader) prefetch_map(&map_a);
+        Ring<C::NA> r;
+        uint32_t it = 0;
         bool ok = true;
         for (uint32_t t = first_tile; ok && t < tiles; t += step) {
             uint32_t i0, j0;
             place(t, &i0, &j0);
-            for (uint32_t k = t0; k < t1; ++k, ++it) {
-                ok = __all_sync(0xffffffffu, mbar_wait(empty(s), phase, guard, kWaitEmpty));
+            for (uint32_t k = t0; k < t1; ++k, ++it, r.next()) {
+                ok = __all_sync(0xffffffffu, mbar_wait(a_empty(r.at), r.phase ^ 1, guard, kWaitAEmpty));
                 if (!ok) break;
                 if (leader) {
-                    const uint32_t dst = base + s * C::stage;
-                    mbar_expect(full(s), C::a_bytes + C::q_bytes);
+                    const uint32_t dst = base + r.at * C::a_bytes;
+                    if (half == 0) mbar_expect(a_full(r.at), C::a_bytes * C::CG);
+                    const uint32_t b = C::CG == 2 ? map_to_rank(a_full(r.at), 0) : a_full(r.at);
+                    auto load = [&](uint32_t to, int32_t x, int32_t y) {
+                        if (C::CG == 2)
+                            tma_load_pair(to, &map_a, x, y, b);
+                        else
+                            tma_load(to, &map_a, x, y, b);
+                    };
                     if (C::A_T) {
-                        tma_load(dst, &map_a, i0, k * kStep, full(s));
-                        tma_load(dst + C::a_bytes / 2, &map_a, i0 + 64, k * kStep, full(s));
+                        load(dst, i0, k * kStep);
+                        load(dst + C::a_bytes / 2, i0 + 64, k * kStep);
                     } else {
-                        tma_load(dst, &map_a, k * kStep, i0, full(s));
+                        load(dst, k * kStep, i0);
                     }
-                    tma_load(dst + C::off_q, &map_q, j0 + half * kSide, k * kStep, full(s));
                 }
                 __syncwarp();
-                if (++s == C::ST) s = 0, phase ^= 1;
             }
         }
-        if (*guard.abort && leader) {  // let copies in flight land before the block retires
+        if (*guard.abort && leader && half == 0) {  // let copies in flight land before the block retires
             const long long c0 = clock64();
-            for (uint32_t i = it > C::ST ? it - C::ST : 0; i < it; ++i)
-                while (!mbar_test(full(i % C::ST), i / C::ST & 1) && clock64() - c0 < kWaitCycles / 8) {
+            for (uint32_t i = it > C::NA ? it - C::NA : 0; i < it; ++i)
+                while (!mbar_test(a_full(i % C::NA), i / C::NA & 1) && clock64() - c0 < kWaitCycles / 8) {
                 }
         }
         __syncwarp();
@@ -217,83 +210,109 @@ __global__ void __launch_bounds__(kThreads, 1)
             // 16 steps of t: 32 bytes of a row, or 16 rows of 128 bytes
             constexpr uint32_t a_next = C::A_T ? 2048 >> 4 : 32 >> 4, b_next = 2048 >> 4;
             const bool leader = elect_one();
-            uint32_t s = 0, phase = 0, b = 0, bphase = 1;
+            Ring<C::NA> ra;
+            Ring<C::NB> rb;
+            Ring<2> rt;
             bool ok = true;
-            for (uint32_t t = first_tile; ok && t < tiles; t += step) {
-                ok = __all_sync(0xffffffffu, mbar_wait<C::CG == 2>(tempty(b), bphase, guard, kWaitTmemEmpty));
+            for (uint32_t t = first_tile; ok && t < tiles; t += step, rt.next()) {
+                ok = __all_sync(0xffffffffu, mbar_wait<C::CG == 2>(tempty(rt.at), rt.phase ^ 1, guard, kWaitTmemEmpty));
                 if (!ok) break;
-                for (uint32_t k = t0; k < t1; ++k) {
-                    ok = __all_sync(0xffffffffu, mbar_wait<C::CG == 2>(ready(s), phase, guard, kWaitConverted));
+                for (uint32_t k = t0; k < t1; ++k, ra.next(), rb.next()) {
+                    ok = mbar_wait(a_full(ra.at), ra.phase, guard, kWaitAFull) &&
+                         mbar_wait<C::CG == 2>(b_full(rb.at), rb.phase, guard, kWaitBFull);
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
                     if (leader) {
-                        const uint32_t src = base + s * C::stage;
-                        const uint64_t da = operand_desc(src, C::A_T ? C::a_bytes / 2 : 16);
-                        const uint64_t db = operand_desc(src + C::off_b, C::b_bytes / 2);
+                        const uint64_t da = operand_desc(base + ra.at * C::a_bytes, C::A_T ? C::a_bytes / 2 : 16);
+                        const uint64_t db = operand_desc(base + C::off_b + rb.at * C::b_bytes, C::b_bytes / 2);
 #pragma unroll
                         for (uint32_t i = 0; i < kStep / 16; ++i)
-                            mma_f16<C::CG>(tmem + b * C::BN, da + i * a_next, db + i * b_next, idesc, k > t0 || i > 0);
-                        mma_commit<C::CG>(empty(s));
-                        if (k + 1 == t1) mma_commit<C::CG>(tfull(b));
+                            mma_f16<C::CG>(tmem + rt.at * C::BN, da + i * a_next, db + i * b_next, idesc,
+                                           k > t0 || i > 0);
+                        mma_commit<C::CG>(a_empty(ra.at));
+                        mma_commit<C::CG>(b_empty(rb.at));
+                        if (k + 1 == t1) mma_commit<C::CG>(tfull(rt.at));
                     }
                     __syncwarp();
-                    if (++s == C::ST) s = 0, phase ^= 1;
                 }
-                b ^= 1;
-                if (b == 0) bphase ^= 1;
             }
         }
     } else if (warp == 2) {
-        uint32_t s = 0, phase = 1;
+        const bool leader = elect_one();
+        if (leader) prefetch_map(&map_q);
+        Ring<C::NQ> r;
+        uint32_t it = 0;
         bool ok = true;
         for (uint32_t t = first_tile; ok && t < tiles; t += step) {
             uint32_t i0, j0;
             place(t, &i0, &j0);
-            const uint32_t jb = j0 / 128 + half;
-            for (uint32_t k = t0; k < t1; ++k) {
-                ok = __all_sync(0xffffffffu, mbar_wait(empty(s), phase, guard, kWaitEmpty));
+            const uint32_t j = j0 + half * kSide, jb = j / 128;
+            for (uint32_t k = t0; k < t1; ++k, ++it, r.next()) {
+                ok = __all_sync(0xffffffffu, mbar_wait(q_empty(r.at), r.phase ^ 1, guard, kWaitQEmpty));
                 if (!ok) break;
-                const uint32_t dst = base + C::off_scale + s * kStep * 4;
+                if (leader) {
+                    mbar_expect(q_full(r.at), C::q_bytes);
+                    tma_load(base + C::off_q + r.at * C::q_bytes, &map_q, j, k * kStep, q_full(r.at));
+                }
+                __syncwarp();
+                const uint32_t dst = base + C::off_scale + r.at * kStep * 4;
 #pragma unroll
                 for (uint32_t i = 0; i < kStep; i += 32) {
-                    const uint32_t r = k * kStep + i + lane;
-                    const bool valid = r < a.nt && jb < a.nb;
-                    cp_async4(dst + (i + lane) * 4, valid ? a.scales + uint64_t(r) * a.nb + jb : a.scales, valid);
+                    const uint32_t row = k * kStep + i + lane;
+                    const bool valid = row < a.nt && jb < a.nb;
+                    cp_async4(dst + (i + lane) * 4, valid ? a.scales + uint64_t(row) * a.nb + jb : a.scales, valid);
                 }
-                cp_async_arrive(full(s));
-                if (++s == C::ST) s = 0, phase ^= 1;
+                cp_async_arrive(q_full(r.at));
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
+        if (*guard.abort && leader) {
+            const long long c0 = clock64();
+            for (uint32_t i = it > C::NQ ? it - C::NQ : 0; i < it; ++i)
+                while (!mbar_test(q_full(i % C::NQ), i / C::NQ & 1) && clock64() - c0 < kWaitCycles / 8) {
+                }
+        }
+        __syncwarp();
     } else if (warp >= 8) {
         const uint32_t mine = (warp - 8) / kGroupWarps, id = threadIdx.x % (kGroupWarps * 32);
         const uint32_t row = id / 2, h = id % 2, swz = row % 8;
-        uint32_t s = 0, phase = 0, turn = 0;
+        Ring<C::NQ> rq;
+        Ring<C::NB> rb;
+        uint32_t turn = 0;
         bool ok = true;
         for (uint32_t t = first_tile; ok && t < tiles; t += step) {
-            for (uint32_t k = t0; k < t1; ++k) {
+            for (uint32_t k = t0; k < t1; ++k, rq.next(), rb.next()) {
                 if (turn == mine) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(full(s), phase, guard, kWaitFull));
+                    ok = mbar_wait(q_full(rq.at), rq.phase, guard, kWaitQFull);
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     // Half a row: 64 columns, four chunks of 16 bytes of Q that
                     // become eight of the operand, each at its place in the
                     // 128-byte swizzle. The two halves take the chunks in
                     // different order, which keeps eight lanes on eight banks.
-                    const uint8_t* q = sm + s * C::stage + C::off_q + row * 128;
-                    uint8_t* d = sm + s * C::stage + C::off_b + h * (C::b_bytes / 2) + row * 128;
-                    const float f = reinterpret_cast<const float*>(sm + C::off_scale)[s * kStep + row];
+                    const uint8_t* q = sm + C::off_q + rq.at * C::q_bytes + row * 128;
+                    uint8_t* d = sm + C::off_b + rb.at * C::b_bytes + h * (C::b_bytes / 2) + row * 128;
+                    const float f = reinterpret_cast<const float*>(sm + C::off_scale)[rq.at * kStep + row];
                     uint4 w[4];
 #pragma unroll
                     for (uint32_t i = 0; i < 4; ++i)
                         w[i] = *reinterpret_cast<const uint4*>(q + (((i ^ 2 * h) + 4 * h) ^ swz) * 16);
+                    uint4 o[8];
 #pragma unroll
                     for (uint32_t i = 0; i < 4; ++i) {
-                        const uint32_t c = 2 * (i ^ 2 * h);
                         const uint2 c0 = convert4(w[i].x, f), c1 = convert4(w[i].y, f);
                         const uint2 c2 = convert4(w[i].z, f), c3 = convert4(w[i].w, f);
-                        *reinterpret_cast<uint4*>(d + (c ^ swz) * 16) = make_uint4(c0.x, c0.y, c1.x, c1.y);
-                        *reinterpret_cast<uint4*>(d + ((c + 1) ^ swz) * 16) = make_uint4(c2.x, c2.y, c3.x, c3.y);
+                        o[2 * i] = make_uint4(c0.x, c0.y, c1.x, c1.y);
+                        o[2 * i + 1] = make_uint4(c2.x, c2.y, c3.x, c3.y);
                     }
+                    ok = mbar_wait(b_empty(rb.at), rb.phase ^ 1, guard, kWaitBEmpty);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive(q_empty(rq.at));
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        *reinterpret_cast<uint4*>(d + ((i ^ 4 * h) ^ swz) * 16) = o[i];
                     fence_async_smem();
                     __syncwarp();
                     // The tensor core of this SM reads what was written here,
@@ -304,41 +323,81 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // global memory, 1300 to 1900 cycles a step.
                     if (lane == 0) {
                         if (C::CG == 2)
-                            mbar_arrive_remote(map_to_rank(ready(s), 0));
+                            mbar_arrive_remote(map_to_rank(b_full(rb.at), 0));
                         else
-                            mbar_arrive(ready(s));
+                            mbar_arrive(b_full(rb.at));
                     }
                 }
                 turn = turn + 1 == kGroups ? 0 : turn + 1;
-                if (++s == C::ST) s = 0, phase ^= 1;
             }
         }
     } else if (warp >= 4) {
         const uint32_t quad = warp % 4, my_lane = quad * 32 + lane;
-        uint32_t b = 0, bphase = 0;
+        const uint32_t stage = C::off_out + quad * C::out_bytes;
+        Ring<2> rt;
         bool ok = true;
-        for (uint32_t t = first_tile; ok && t < tiles; t += step) {
+        for (uint32_t t = first_tile; ok && t < tiles; t += step, rt.next()) {
             uint32_t i0, j0;
             place(t, &i0, &j0);
-            ok = __all_sync(0xffffffffu, mbar_wait(tfull(b), bphase, guard, kWaitTmemFull));
+            ok = __all_sync(0xffffffffu, mbar_wait(tfull(rt.at), rt.phase, guard, kWaitTmemFull));
             __syncwarp();
             if (!ok) break;
             tc_fence_after();
-            const uint32_t row = i0 + my_lane;
+            const uint32_t row0 = i0 + quad * 32;
             const bool share = C::CG == 1 && a.split > 1;
 #pragma unroll 1
             for (uint32_t c = 0; c < C::BN; c += 32) {
                 uint32_t v[32];
-                tmem_ld(tmem + b * C::BN + c + (quad * 32 << 16), v);
+                tmem_ld(tmem + rt.at * C::BN + c + (quad * 32 << 16), v);
                 tmem_ld_keep(v);
                 if (share) {
-                    // Partial sums meet in shared memory: the stages are free
+                    // Partial sums meet in shared memory: the rings are free
                     // (the last product is done, one tile to a CTA).
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         reinterpret_cast<uint32_t*>(sm)[(c + i) * kSide + my_lane] = v[i];
-                } else if (row < a.ni && j0 + c < a.nj) {
-                    store_row(a, row, j0 + c, v);
+                } else if (row0 >= a.ni || j0 + c >= a.nj) {
+                    // nothing of this piece is inside
+                } else if (a.tiled) {
+                    // Through shared memory (in the 64-byte swizzle) and out as
+                    // tiles: a lane's own stores would each touch a line of
+                    // their own, and hold up the converters' traffic.
+                    const uint32_t at = lane * 64, swz = lane / 2 % 4;
+                    if (a.type == 2) {
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            if (lane == 0) tma_store_wait_read();
+                            __syncwarp();
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; ++i)
+                                *reinterpret_cast<uint4*>(sm + stage + at + (i ^ swz) * 16) = make_uint4(
+                                    v[16 * p + 4 * i], v[16 * p + 4 * i + 1], v[16 * p + 4 * i + 2], v[16 * p + 4 * i + 3]);
+                            fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0 && j0 + c + 16 * p < a.nj)
+                                tma_store(&map_out, base + stage, j0 + c + 16 * p, row0);
+                        }
+                    } else {
+                        if (lane == 0) tma_store_wait_read();
+                        __syncwarp();
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                w[k] = pack16(a.type, __uint_as_float(v[8 * i + 2 * k]),
+                                              __uint_as_float(v[8 * i + 2 * k + 1]));
+                            *reinterpret_cast<uint4*>(sm + stage + at + (i ^ swz) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) tma_store(&map_out, base + stage, j0 + c, row0);
+                    }
+                } else if (row0 + lane < a.ni) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 32; ++i)
+                        if (j0 + c + i < a.nj)
+                            store_one(a, int64_t(row0 + lane) * a.ld + j0 + c + i, __uint_as_float(v[i]));
                 }
                 __syncwarp();
             }
@@ -346,13 +405,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) {
                 if (C::CG == 2)
-                    mbar_arrive_remote(map_to_rank(tempty(b), 0));
+                    mbar_arrive_remote(map_to_rank(tempty(rt.at), 0));
                 else
-                    mbar_arrive(tempty(b));
+                    mbar_arrive(tempty(rt.at));
             }
-            b ^= 1;
-            if (b == 0) bphase ^= 1;
         }
+        if (lane == 0) tma_store_wait();
     }
     __syncwarp();
     if (C::CG == 1 && a.split > 1) {
@@ -385,10 +443,18 @@ cudaError_t run(MatIn dy, int64_t dy_rows, int64_t dy_cols, const Block128In& q,
     Args a{};
     cudaError_t e = error_word(&a.error);
     if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(k_grad<C>), C::smem);
-    CUtensorMap ma, mq;
+    CUtensorMap ma, mq, mo;
     if (e == cudaSuccess)
         e = tile_map(&ma, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dy.ptr, dy_cols, dy_rows, dy.ld * 2, 64,
                      C::A_T ? kStep : kSide);
+    const int64_t esz = type == FloatType::kFp32 ? 4 : 2;
+    a.tiled = reinterpret_cast<uintptr_t>(out.ptr) % 16 == 0 && out.ld * esz % 16 == 0;
+    mo = ma;
+    if (e == cudaSuccess && a.tiled)
+        e = tile_map(&mo, type == FloatType::kBf16   ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                          : type == FloatType::kFp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                     out.ptr, nj, ni, out.ld * esz, uint32_t(64 / esz), 32, 64);
     if (e == cudaSuccess) e = tile_map(&mq, CU_TENSOR_MAP_DATA_TYPE_UINT8, q.q, nj, nt, q.ld, kSide, kStep);
     if (e != cudaSuccess) return e;
     a.scales = q.scales;
@@ -402,8 +468,6 @@ cudaError_t run(MatIn dy, int64_t dy_rows, int64_t dy_cols, const Block128In& q,
     a.tiles_j = uint32_t((nj + C::BN - 1) / C::BN);
     a.split = C::CG == 2 ? 1 : split;
     a.type = int(type);
-    const int64_t esz = type == FloatType::kFp32 ? 4 : 2;
-    a.vec = reinterpret_cast<uintptr_t>(out.ptr) % 16 == 0 && out.ld * esz % 16 == 0;
     const uint64_t tiles = uint64_t(a.tiles_i) * a.tiles_j;
     if (tiles * a.split > 0x7fffffff) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
@@ -421,7 +485,7 @@ cudaError_t run(MatIn dy, int64_t dy_rows, int64_t dy_cols, const Block128In& q,
     }
     const uint64_t units = a.split > 1 ? tiles : std::min<uint64_t>(tiles, uint64_t(sm_count()) / group);
     cfg.gridDim = dim3(uint32_t(units * group));
-    e = cudaLaunchKernelEx(&cfg, k_grad<C>, ma, mq, a);
+    e = cudaLaunchKernelEx(&cfg, k_grad<C>, ma, mq, mo, a);
     g_block128_launches.fetch_add(1, std::memory_order_relaxed);
     return e != cudaSuccess ? e : cudaGetLastError();
 }

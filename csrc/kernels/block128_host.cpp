@@ -73,14 +73,15 @@ EncodeTiled encode_tiled() {
 }  // namespace
 
 cudaError_t tile_map(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, int64_t cols, int64_t rows,
-                     int64_t pitch, uint32_t box_cols, uint32_t box_rows, bool swizzle) {
+                     int64_t pitch, uint32_t box_cols, uint32_t box_rows, int swizzle) {
     const EncodeTiled fn = encode_tiled();
     if (!fn) return cudaErrorNotSupported;
     const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
     const cuuint64_t strides[1] = {cuuint64_t(pitch)};
     const cuuint32_t box[2] = {box_cols, box_rows}, step[2] = {1, 1};
     const CUresult r = fn(map, type, 2, const_cast<void*>(ptr), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                          swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                          : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;

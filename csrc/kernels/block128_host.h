@@ -13,10 +13,10 @@ namespace kern {
 extern std::atomic<uint64_t> g_block128_launches;
 
 // Tensor map of a row-major [rows, cols] matrix with `pitch` bytes a row, read
-// in tiles of box_rows x box_cols (in the 128-byte swizzle unless told
-// otherwise); what lies outside reads as 0.
+// in tiles of box_rows x box_cols in a swizzle of 128, 64 or 0
+// bytes; what lies outside reads as 0.
 cudaError_t tile_map(CUtensorMap* map, CUtensorMapDataType type, const void* ptr, int64_t cols, int64_t rows,
-                     int64_t pitch, uint32_t box_cols, uint32_t box_rows, bool swizzle = true);
+                     int64_t pitch, uint32_t box_cols, uint32_t box_rows, int swizzle = 128);
 
 // This device's error word: host-mapped, 0 until a bounded wait of a kernel
 // runs out. block128_error() returns it without waiting for anything.

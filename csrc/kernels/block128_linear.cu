@@ -413,7 +413,7 @@ cudaError_t run(const Problem& p, uint32_t split) {
         e = tile_map(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.kept.q, p.k, p.m, p.kept.ld, kBlock, C::BN / C::CG);
     if (e == cudaSuccess)
         e = tile_map(&msx, CU_TENSOR_MAP_DATA_TYPE_UINT32, p.work, ts.stride, int64_t(a.tiles_m) * a.nb,
-                     int64_t(ts.stride) * 4, ts.stride, 1, false);
+                     int64_t(ts.stride) * 4, ts.stride, 1, 0);
     if (e == cudaSuccess) e = quantize_for_tiles(p.x, p.xtype, p.kept, ts, p.m, p.k, p.s);
     if (e != cudaSuccess) return e;
     a.scale_w = p.w.scales;
