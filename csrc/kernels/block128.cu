@@ -191,7 +191,14 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // exp of the negative side alone: 1 / (1 + exp(-g)) would be 0 below g = -88.7, where g s(g) is still in range.
+// Results in 16 bits take the hardware's exp and reciprocal, whose errors (2^-22 and a unit for each of g's) are far
+// under half a step of theirs, 2^-12 and more; in fp32 they would be the largest error, so fp32 takes the exact forms.
+template <typename T>
 __device__ __forceinline__ float sigmoid(float g) {
+    if (sizeof(T) == 2) {
+        const float e = __expf(-fabsf(g));
+        return __fdividef(g >= 0.f ? 1.f : e, 1.f + e);
+    }
     const float e = expf(-fabsf(g));
     return (g >= 0.f ? 1.f : e) / (1.f + e);
 }
@@ -207,7 +214,7 @@ __global__ void __launch_bounds__(kThreads)
         load8<T, VEC>(gate + p.row * ldg, p.c, p.n, g);
         load8<T, VEC>(up + p.row * ldu, p.c, p.n, u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = g[i] * sigmoid(g[i]) * u[i];
+        for (int i = 0; i < 8; ++i) o[i] = g[i] * sigmoid<T>(g[i]) * u[i];
         store8<T, VEC>(h + p.row * ldh, p.c, p.n, o);
         const bool first = (threadIdx.x & 15) == 0 && blk < sh.total;
         uint2 v = quantize8(g, &s);
@@ -239,7 +246,7 @@ __global__ void __launch_bounds__(kThreads)
         fp8_to_float(vu.y, u + 4);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float gi = g[i] * fg, ui = u[i] * fu, s = sigmoid(gi);
+            const float gi = g[i] * fg, ui = u[i] * fu, s = sigmoid<T>(gi);
             b[i] = d[i] * gi * s;
             a[i] = d[i] * ui * s * (1.f + gi * (1.f - s));
         }

@@ -29,11 +29,17 @@ _FP8 = torch.float8_e4m3fn
 _TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
+# The current stream and device as plain numbers: torch.cuda's functions build
+# objects, which at the smallest sizes takes longer than the kernels.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
 def _type(dtype: torch.dtype, what: str) -> int:
-    try:
-        return _TYPE[dtype]
-    except KeyError:
-        raise ValueError(f"{what} must be bfloat16, float16 or float32; got {dtype}") from None
+    code = _TYPE.get(dtype)
+    if code is None:
+        raise ValueError(f"{what} must be bfloat16, float16 or float32; got {dtype}")
+    return code
 
 
 def _on_gpu(t, what: str) -> torch.Tensor:
@@ -44,35 +50,45 @@ def _on_gpu(t, what: str) -> torch.Tensor:
     return t
 
 
-def _same_device(dev: torch.device, **tensors) -> None:
-    for what, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{what} is on {t.device}, the first operand on {dev}")
+def _same_device(first: torch.Tensor, t: torch.Tensor, what: str) -> None:
+    if t.get_device() != first.get_device():
+        raise ValueError(f"{what} is on {t.device}, the first operand on {first.device}")
+
+
+def _launch(device: int, fn, *args) -> None:
+    """``fn(*args, stream)`` on the device's current stream, with the device current."""
+    if device == _current_device():
+        fn(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            fn(*args, _raw_stream(device))
 
 
 def _matrix(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
     """(2-D form with unit column stride, rows, cols, pitch): a view where the strides allow one."""
-    if t.dim() == 0:
-        raise ValueError(f"{what} must have at least one dimension")
-    cols = t.shape[-1]
     if t.dim() != 2:
+        if t.dim() == 0:
+            raise ValueError(f"{what} must have at least one dimension")
+        cols = t.shape[-1]
         t = t.reshape(t.numel() // cols if cols else 0, cols)
-    rows = t.shape[0]
-    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
+    rows, cols = t.shape
+    pitch, one = t.stride()
+    if (cols > 1 and one != 1) or (rows > 1 and pitch < cols):
         t = t.contiguous()
-    return t, rows, cols, t.stride(0) if rows > 1 else cols
+        pitch = cols
+    return t, rows, cols, pitch if rows > 1 else cols
 
 
 def _tiled(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
     """``_matrix`` whose base and pitch are multiples of 16 bytes, as the tile copies need: a copy if they are not."""
     t, rows, cols, ld = _matrix(t, what)
     per = 16 // t.element_size()
-    pitch = -(-cols // per) * per
     if rows == 1:
-        ld = pitch
+        ld = -(-cols // per) * per
     if ld % per or t.data_ptr() % 16:
-        p = torch.empty((rows, pitch), dtype=t.dtype, device=t.device)[:, :cols]
-        t, ld = p.copy_(t), pitch
+        ld = -(-cols // per) * per
+        p = torch.empty((rows, ld), dtype=t.dtype, device=t.device)[:, :cols]
+        t = p.copy_(t)
     return t, rows, cols, ld
 
 
@@ -80,46 +96,28 @@ def _pair(p, what: str):
     """(q, scales, rows, cols, pitch) of a block-128 pair."""
     if not isinstance(p, (tuple, list)) or len(p) != 2:
         raise TypeError(f"{what} must be a (q, scales) pair")
-    q, scales = _on_gpu(p[0], f"{what}: q"), _on_gpu(p[1], f"{what}: scales")
+    q, scales = p
+    _on_gpu(q, what)
+    _on_gpu(scales, what)
     if q.dtype != _FP8:
         raise ValueError(f"{what}: q must be float8_e4m3fn; got {q.dtype}")
     if scales.dtype != torch.float32:
         raise ValueError(f"{what}: scales must be float32; got {scales.dtype}")
-    _same_device(q.device, scales=scales)
-    q, rows, cols, ld = _tiled(q, f"{what}: q")
+    _same_device(q, scales, what)
+    q, rows, cols, ld = _tiled(q, what)
     if scales.numel() != rows * -(-cols // BLOCK):
         raise ValueError(f"{what}: {tuple(scales.shape)} scales do not fit {rows} rows of {cols} values: one for "
                          f"each {BLOCK} values of a row")
-    return q, scales.contiguous(), rows, cols, ld
+    return q, scales if scales.is_contiguous() else scales.contiguous(), rows, cols, ld
 
 
-def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
-class _on:
-    """The device as the current one, for as long as it takes; costs nothing when it already is."""
-
-    def __init__(self, dev: torch.device):
-        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-
-
-def _empty_pair(shape, dev: torch.device):
-    """Uninitialised (q, scales) for values of `shape`, and q's pitch."""
-    cols = shape[-1]
+def _empty_pair(lead, cols: int, dev: torch.device):
+    """Uninitialised (q, scales) of [*lead, cols] values, and q's pitch."""
     pitch = -(-cols // 16) * 16
-    q = torch.empty((*shape[:-1], pitch), dtype=_FP8, device=dev)
+    q = torch.empty((*lead, pitch), dtype=_FP8, device=dev)
     if pitch != cols:
         q = q[..., :cols]
-    return (q, torch.empty((*shape[:-1], -(-cols // BLOCK)), dtype=torch.float32, device=dev)), pitch
+    return (q, torch.empty((*lead, -(-cols // BLOCK)), dtype=torch.float32, device=dev)), pitch
 
 
 def quantize(x: torch.Tensor) -> Block128:
@@ -129,14 +127,13 @@ def quantize(x: torch.Tensor) -> Block128:
     The scale is the smallest power of two (at least 2^-117) that brings a block within e4m3's 448, 1 for a block
     of zeros, so the only rounding is e4m3's (to nearest, ties to even). A value that is not finite becomes NaN and
     does not count in its block's scale."""
-    x = _on_gpu(x.detach() if isinstance(x, torch.Tensor) else x, "x")
+    _on_gpu(x, "x")
     code = _type(x.dtype, "x")
-    shape = x.shape
+    lead = x.shape[:-1]
     x, rows, cols, ld = _matrix(x, "x")
-    (q, scales), pitch = _empty_pair(shape, x.device)
-    with _on(x.device):
-        native().k_quantize_block128(x.data_ptr(), ld, code, q.data_ptr(), pitch, scales.data_ptr(), rows, cols,
-                                     _stream(x.device))
+    (q, scales), pitch = _empty_pair(lead, cols, x.device)
+    _launch(x.get_device(), native().k_quantize_block128, x.data_ptr(), ld, code, q.data_ptr(), pitch,
+            scales.data_ptr(), rows, cols)
     return q, scales
 
 
@@ -146,9 +143,8 @@ def dequantize(x: Block128, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor
     code = _type(dtype, "dtype")
     q, scales, rows, cols, ld = _pair(x, "x")
     out = torch.empty(x[0].shape, dtype=dtype, device=q.device)
-    with _on(q.device):
-        native().k_dequantize_block128(q.data_ptr(), ld, scales.data_ptr(), out.data_ptr(), cols, code, rows, cols,
-                                       _stream(q.device))
+    _launch(q.get_device(), native().k_dequantize_block128, q.data_ptr(), ld, scales.data_ptr(), out.data_ptr(), cols,
+            code, rows, cols)
     return out
 
 
@@ -196,32 +192,31 @@ def _forward(x, weight, bias, out_dtype, keep: bool):
     if x.dim() == 0 or x.shape[-1] != k:
         raise ValueError(f"x has shape {tuple(x.shape)}, the weight {k} columns")
     lead = x.shape[:-1]
-    x, m, _, ldx = _matrix(x.detach(), "x")
+    x, m, _, ldx = _matrix(x, "x")
     dev = x.device
-    _same_device(dev, weight=wq, bias=bias)
+    _same_device(x, wq, "weight")
     if bias is not None:
+        _same_device(x, bias, "bias")
         if bias.shape != (n,):
             raise ValueError(f"bias must have shape ({n},); got {tuple(bias.shape)}")
         if bias.dtype != out_dtype:
             raise ValueError(f"bias must be {out_dtype} like the result; got {bias.dtype}")
-        bias = bias.detach().contiguous()
+        bias = bias.contiguous()
     y = torch.empty((*lead, n), dtype=out_dtype, device=dev)
     if k == 0:
         return (y.zero_() if bias is None else y.copy_(bias.expand_as(y))), quantize(x) if keep else None, wp
     C = native()
     work_bytes = C.linear_work_bytes(m, k)
     if keep:
-        (q, scales), pitch = _empty_pair((m, k), dev)
+        (q, scales), pitch = _empty_pair((m,), k, dev)
         work = torch.empty(work_bytes, dtype=torch.uint8, device=dev)
         ptrs = q.data_ptr(), pitch, scales.data_ptr(), work.data_ptr()
     else:
         pitch = -(-k // 16) * 16
         work = torch.empty(work_bytes + m * pitch, dtype=torch.uint8, device=dev)
         ptrs = work.data_ptr() + work_bytes, pitch, 0, work.data_ptr()
-    with _on(dev):
-        C.k_linear_block128(x.data_ptr(), ldx, _TYPE[x.dtype], *ptrs, work_bytes, wq.data_ptr(), ldw, ws.data_ptr(),
-                            0 if bias is None else bias.data_ptr(), y.data_ptr(), n, _TYPE[out_dtype], m, n, k,
-                            _stream(dev))
+    _launch(x.get_device(), C.k_linear_block128, x.data_ptr(), ldx, _TYPE[x.dtype], *ptrs, work_bytes, wq.data_ptr(),
+            ldw, ws.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr(), n, _TYPE[out_dtype], m, n, k)
     return y, (q, scales) if keep else None, wp
 
 
@@ -230,8 +225,8 @@ def _gradient(dy: torch.Tensor, other: Block128, what: str):
     if dy.dtype != torch.bfloat16:
         raise ValueError(f"dy must be bfloat16; got {dy.dtype}")
     p = _pair(other, what)
-    _same_device(dy.device, **{what: p[0]})
-    return _tiled(dy.detach(), "dy"), p
+    _same_device(dy, p[0], what)
+    return _tiled(dy, "dy"), p
 
 
 def linear_input_grad(dy: torch.Tensor, weight: Block128, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -244,9 +239,8 @@ def linear_input_grad(dy: torch.Tensor, weight: Block128, out_dtype: torch.dtype
     dx = torch.empty((*dy.shape[:-1], k), dtype=out_dtype, device=d.device)
     if n == 0:
         return dx.zero_()
-    with _on(d.device):
-        native().k_matmul_input_grad(d.data_ptr(), ldd, q.data_ptr(), ld, scales.data_ptr(), dx.data_ptr(), k, code,
-                                     m, n, k, _stream(d.device))
+    _launch(d.get_device(), native().k_matmul_input_grad, d.data_ptr(), ldd, q.data_ptr(), ld, scales.data_ptr(),
+            dx.data_ptr(), k, code, m, n, k)
     return dx
 
 
@@ -260,9 +254,8 @@ def linear_weight_grad(dy: torch.Tensor, x: Block128, out_dtype: torch.dtype = t
     dw = torch.empty((n, k), dtype=out_dtype, device=d.device)
     if m == 0:
         return dw.zero_()
-    with _on(d.device):
-        native().k_matmul_weight_grad(d.data_ptr(), ldd, q.data_ptr(), ld, scales.data_ptr(), dw.data_ptr(), k, code,
-                                      m, n, k, _stream(d.device))
+    _launch(d.get_device(), native().k_matmul_weight_grad, d.data_ptr(), ldd, q.data_ptr(), ld, scales.data_ptr(),
+            dw.data_ptr(), k, code, m, n, k)
     return dw
 
 
@@ -295,24 +288,21 @@ class _Linear(torch.autograd.Function):
 def swiglu_forward(gate: torch.Tensor, up: torch.Tensor):
     """``silu(gate) * up`` and what its backward pass keeps: ``(h, (kept_gate, kept_up))``, two pairs as ``quantize``
     makes them. ``h`` is computed from the unquantised inputs."""
-    gate, up = (t.detach() if isinstance(t, torch.Tensor) else t for t in (gate, up))
     _on_gpu(gate, "gate")
     _on_gpu(up, "up")
     code = _type(gate.dtype, "gate")
-    if up.dtype != gate.dtype or up.shape != gate.shape:
-        raise ValueError(f"up ({tuple(up.shape)}, {up.dtype}) must match gate ({tuple(gate.shape)}, {gate.dtype})")
-    dev = gate.device
-    _same_device(dev, up=up)
     shape = gate.shape
+    if up.dtype != gate.dtype or up.shape != shape:
+        raise ValueError(f"up ({tuple(up.shape)}, {up.dtype}) must match gate ({tuple(shape)}, {gate.dtype})")
+    _same_device(gate, up, "up")
+    dev = gate.device
     g, rows, cols, ldg = _matrix(gate, "gate")
     u, _, _, ldu = _matrix(up, "up")
     h = torch.empty(shape, dtype=gate.dtype, device=dev)
-    kg, pitch = _empty_pair(shape, dev)
-    ku, _ = _empty_pair(shape, dev)
-    with _on(dev):
-        native().k_swiglu_forward(g.data_ptr(), ldg, u.data_ptr(), ldu, code, h.data_ptr(), cols, kg[0].data_ptr(),
-                                  kg[1].data_ptr(), ku[0].data_ptr(), ku[1].data_ptr(), pitch, rows, cols,
-                                  _stream(dev))
+    kg, pitch = _empty_pair(shape[:-1], cols, dev)
+    ku, _ = _empty_pair(shape[:-1], cols, dev)
+    _launch(g.get_device(), native().k_swiglu_forward, g.data_ptr(), ldg, u.data_ptr(), ldu, code, h.data_ptr(), cols,
+            kg[0].data_ptr(), kg[1].data_ptr(), ku[0].data_ptr(), ku[1].data_ptr(), pitch, rows, cols)
     return h, (kg, ku)
 
 
@@ -325,16 +315,16 @@ def swiglu_backward(dh: torch.Tensor, kept) -> Tuple[torch.Tensor, torch.Tensor]
         raise TypeError("kept must be the two pairs that swiglu_forward returned")
     gq, gs, rows, cols, ldg = _pair(kept[0], "kept gate")
     uq, us, rows_u, cols_u, ldu = _pair(kept[1], "kept up")
-    d, rows_d, cols_d, ldd = _matrix(dh.detach(), "dh")
+    d, rows_d, cols_d, ldd = _matrix(dh, "dh")
     if (rows, cols) != (rows_u, cols_u) or (rows, cols) != (rows_d, cols_d):
         raise ValueError(f"dh has shape {tuple(dh.shape)}, the kept pairs {tuple(kept[0][0].shape)} and "
                          f"{tuple(kept[1][0].shape)}")
-    dev = d.device
-    _same_device(dev, gate=gq, up=uq)
-    dg, du = (torch.empty(dh.shape, dtype=dh.dtype, device=dev) for _ in range(2))
-    with _on(dev):
-        native().k_swiglu_backward(d.data_ptr(), ldd, code, gq.data_ptr(), ldg, gs.data_ptr(), uq.data_ptr(), ldu,
-                                   us.data_ptr(), dg.data_ptr(), du.data_ptr(), cols, rows, cols, _stream(dev))
+    _same_device(d, gq, "kept gate")
+    _same_device(d, uq, "kept up")
+    dg = torch.empty(dh.shape, dtype=dh.dtype, device=d.device)
+    du = torch.empty(dh.shape, dtype=dh.dtype, device=d.device)
+    _launch(d.get_device(), native().k_swiglu_backward, d.data_ptr(), ldd, code, gq.data_ptr(), ldg, gs.data_ptr(),
+            uq.data_ptr(), ldu, us.data_ptr(), dg.data_ptr(), du.data_ptr(), cols, rows, cols)
     return dg, du
 
 
