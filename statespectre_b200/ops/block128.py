@@ -25,6 +25,7 @@ from .._native import native
 Block128 = Tuple[torch.Tensor, torch.Tensor]
 
 BLOCK = 128
+_MOST = 1 << 31  # a row pitch from here on is copied away
 _FP8 = torch.float8_e4m3fn
 _TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
@@ -73,7 +74,7 @@ def _matrix(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
         t = t.reshape(t.numel() // cols if cols else 0, cols)
     rows, cols = t.shape
     pitch, one = t.stride()
-    if (cols > 1 and one != 1) or (rows > 1 and pitch < cols):
+    if (cols > 1 and one != 1) or (rows > 1 and not cols <= pitch < _MOST):
         t = t.contiguous()
         pitch = cols
     return t, rows, cols, pitch if rows > 1 else cols
