@@ -69,12 +69,12 @@ struct Config {
     static constexpr uint32_t smem = off_misc + 16 + 1024;  // + alignment of the base
     static constexpr int CPT = BN / (EW / 4);                  // columns of one epilogue thread
     static constexpr int CH = CPT % 32 ? 16 : 32;            // columns of one tensor-memory load
-    // The epilogue either reads all its columns of a product at once, which
-    // frees the buffer before the arithmetic, or two loads in turn where there
-    // are no registers for that. The first form of eight warps needs more
-    // registers than an even share: the four other warps give up theirs.
-    static constexpr bool ALL = EW == 8 || CPT <= 32;
-    static constexpr bool SHIFT = EW == 8;
+    // The epilogue reads all its columns of a product before the arithmetic, so
+    // that the buffer is free early.
+    // 224 columns a pair take more registers for that than an even share: the
+    // four warps that are not the epilogue give up theirs.
+    static constexpr bool SHIFT = CPT > 64;
+    static_assert(!SHIFT || EW == 8, "");
     static constexpr int kEven = 168, kFew = 40, kMany = 232;
     static_assert(!SHIFT || 128 * kFew + 256 * kMany <= 384 * kEven, "a split that the block has registers for");
     static_assert(tmem_used <= 512 && tmem_cols * per_sm <= 512, "tensor memory");
@@ -158,7 +158,10 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
     if (warp >= 4 && warp < 8) tmem_fill4(tmem + C::tmem_sw + (warp % 4 * 32 << 16), 0x7f7f7f7fu);  // e8m0 of 1
     tc_fence_before();
     __syncthreads();
-    if (C::CG == 2 || a.split > 1) cluster_sync();
+    if (C::CG == 2)
+        cluster_sync();
+    else if (a.split > 1)
+        cluster_arrive();  // waited for where the parts meet
     tc_fence_after();
 
     // Tiles in groups of 16 row tiles of w, those fastest: what is in flight
@@ -174,13 +177,35 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
         if (C::SHIFT) regs_less<C::kFew>();
         if (warp == 0) {
             const bool leader = elect_one();
-            if (leader) {
-                prefetch_map(&map_w);
-                prefetch_map(&map_x);
-                prefetch_map(&map_sx);
-            }
             uint32_t it = 0, s = 0, phase = 1;
             bool ok = true;
+            auto load_w = [&](uint32_t s, uint32_t kb, uint32_t n0) {
+                const uint32_t dst = base + s * C::stage_pitch;
+                if (C::CG == 1) {
+                    mbar_expect(full(s), C::stage_bytes);
+                    tma_load(dst, &map_w, kb * kBlock, n0, full(s));
+                } else {
+                    // The tiles of both CTAs count on the first one's barrier,
+                    // where the products wait.
+                    if (half == 0) mbar_expect(full(s), 2 * C::stage_bytes);
+                    tma_load_pair(dst, &map_w, kb * kBlock, n0, map_to_rank(full(s), 0));
+                }
+            };
+            // The first tiles of w do not wait for x's quantisation.
+            uint32_t ahead = 0;
+            if (first_tile < tiles) {
+                uint32_t n0, tm;
+                place(first_tile, &n0, &tm);
+                ahead = min(kb1 - kb0, uint32_t(C::ST));
+                if (leader) {
+                    prefetch_map(&map_w);
+                    prefetch_map(&map_x);
+                    prefetch_map(&map_sx);
+                    for (uint32_t i = 0; i < ahead; ++i) load_w(i, kb0 + i, n0);
+                }
+                __syncwarp();
+            }
+            grid_wait();
             for (uint32_t t = first_tile; ok && t < tiles; t += step) {
                 uint32_t n0, tm;
                 place(t, &n0, &tm);
@@ -188,21 +213,16 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                     ok = __all_sync(0xffffffffu, mbar_wait(empty(s), phase, guard, kWaitEmpty));
                     if (!ok) break;
                     if (leader) {
-                        const uint32_t dst = base + s * C::stage_pitch, dst_sx = dst + C::w_bytes + C::x_bytes;
+                        if (it >= ahead) load_w(s, kb, n0);
+                        const uint32_t dst = base + s * C::stage_pitch + C::w_bytes, dst_sx = dst + C::x_bytes;
                         if (C::CG == 1) {
-                            mbar_expect(full(s), C::stage_bytes);
-                            tma_load(dst, &map_w, kb * kBlock, n0, full(s));
-                            tma_load(dst + C::w_bytes, &map_x, kb * kBlock, tm * C::BN, full(s));
+                            tma_load(dst, &map_x, kb * kBlock, tm * C::BN, full(s));
                             tma_load(dst_sx, &map_sx, 0, tm * a.nb + kb, full(s));
                         } else {
-                            // The tiles of both CTAs count on the first one's
-                            // barrier, where the products wait. Both need all
-                            // of the factors, which go from each CTA's own
-                            // shared memory to its own tensor memory.
-                            if (half == 0) mbar_expect(full(s), 2 * C::stage_bytes);
+                            // Both CTAs need all of the factors, which go from
+                            // each one's shared memory to its tensor memory.
                             const uint32_t b = map_to_rank(full(s), 0);
-                            tma_load_pair(dst, &map_w, kb * kBlock, n0, b);
-                            tma_load_pair(dst + C::w_bytes, &map_x, kb * kBlock, tm * C::BN + half * (C::BN / 2), b);
+                            tma_load_pair(dst, &map_x, kb * kBlock, tm * C::BN + half * (C::BN / 2), b);
                             tma_load_pair(dst_sx, &map_sx, 0, tm * a.nb + kb, b);
                         }
                     }
@@ -287,40 +307,20 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                 tc_fence_after();
                 const uint32_t from = tmem + b * C::BN + mine + (quad * 32 << 16);
                 constexpr int NC = C::CPT / C::CH;
-                uint32_t v[C::ALL ? NC : 2][C::CH];
-                auto add = [&](int c) {
-                    uint32_t(&w)[C::CH] = v[C::ALL ? c : c & 1];
+                uint32_t v[NC][C::CH];
 #pragma unroll
-                    for (int i = 0; i < C::CH; ++i) add_scaled(acc[c * C::CH + i], w[i], scale);
-                };
-                auto release = [&] {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (C::CG == 2)
-                            mbar_arrive_remote(map_to_rank(tempty(b), 0));
-                        else
-                            mbar_arrive(tempty(b));
-                    }
-                };
-                if (C::ALL) {
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) tmem_ld(from + c * C::CH, v[C::ALL ? c : 0]);
-                    tmem_ld_wait();
-                    release();
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) add(c);
-                } else {
-                    tmem_ld(from, v[0]);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        if (c + 1 < NC) tmem_ld(from + (c + 1) * C::CH, v[C::ALL ? 0 : (c + 1) & 1]);
-                        add(c);
-                        if (c + 1 < NC) tmem_ld_wait();
-                    }
-                    release();
+                for (int c = 0; c < NC; ++c) tmem_ld(from + c * C::CH, v[c]);
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (C::CG == 2)
+                        mbar_arrive_remote(map_to_rank(tempty(b), 0));
+                    else
+                        mbar_arrive(tempty(b));
                 }
+#pragma unroll
+                for (int i = 0; i < C::CPT; ++i) add_scaled(acc[i], v[i / C::CH][i % C::CH], scale);
             }
             if (C::CG == 1 && a.split > 1) {
                 // Partial sums meet in shared memory: the stages are free (the
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                 // the columns, in the order of the parts.
                 float* part_sum = reinterpret_cast<float*>(sm);
 #pragma unroll
-                for (int i = 0; i < C::CPT; ++i) part_sum[i * kLanes + my_lane] = acc[i];
+                for (int i = 0; i < C::CPT; ++i) part_sum[(mine + i) * kLanes + my_lane] = acc[i];
                 break;
             }
             // The lanes past the last row take no other way through the loop:
@@ -354,6 +354,7 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
     }
     if (C::CG == 1 && a.split > 1) {
         __syncthreads();
+        cluster_wait();
         cluster_sync();
         uint32_t n0, tm;
         place(first_tile, &n0, &tm);
@@ -427,7 +428,7 @@ cudaError_t run(const Problem& p, uint32_t split) {
     const uint64_t tiles = uint64_t(a.tiles_n) * a.tiles_m;
     if (tiles * a.split > 0x7fffffff) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     cfg.blockDim = dim3(C::threads);
     cfg.dynamicSmemBytes = C::smem;
     cfg.stream = p.s;
@@ -439,6 +440,10 @@ cudaError_t run(const Problem& p, uint32_t split) {
         at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
         cfg.numAttrs = 1;
     }
+    // starts while x is being quantised, with what does not need it (3 us of a decode step)
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
     // a split tile has a cluster of its own; else the CTAs (or pairs) walk the tiles
     const uint64_t units = a.split > 1 ? tiles : std::min<uint64_t>(tiles, uint64_t(sm_count()) * C::per_sm / group);
     cfg.gridDim = dim3(uint32_t(units * group));
@@ -469,15 +474,15 @@ cudaError_t linear_block128(MatIn x, FloatType xtype, Block128Out kept, void* wo
         return cudaErrorInvalidValue;
     if (m == 0) return cudaSuccess;
     if (n == 0) return kept.scales ? quantize_block128(x, xtype, kept, m, k, s) : cudaSuccess;
-    if (!x.ptr || x.ld < k || !q_ok(w, k) || !y.ptr || y.ld < n || !work || (reinterpret_cast<uintptr_t>(work) & 15))
+    if (!x.ptr || x.ld < k || int(xtype) < 0 || int(xtype) > 2 || !q_ok(w, k) || !y.ptr || y.ld < n || !work || (reinterpret_cast<uintptr_t>(work) & 15))
         return cudaErrorInvalidValue;
     const Problem p{x, xtype, kept, static_cast<uint32_t*>(work), work_bytes, w, bias, y, type, m, n, k, s};
     const int64_t nb = (k + 127) / 128, nt = (n + 127) / 128;
     if (m <= 16) return run<Config<16, 1, 4, 5, 4, 2>>(p, parts(nt, nb, 2));
     if (m <= 32) return run<Config<32, 1, 4, 5, 4, 2>>(p, parts(nt, nb, 2));
-    if (m <= 64) return run<Config<64, 1, 4, 4, 3, 2>>(p, parts(nt, nb, 2));
+    if (m <= 64) return run<Config<64, 1, 8, 8, 4, 1>>(p, parts(nt, nb, 1));
     if (((m + 223) / 224) * ((n + 255) / 256) >= 74) return run<Config<224, 2, 8, 6, 2, 1>>(p, 1);
-    return run<Config<128, 1, 4, 6, 2, 1>>(p, parts((m + 127) / 128 * nt, nb, 1));
+    return run<Config<128, 1, 8, 6, 3, 1>>(p, parts((m + 127) / 128 * nt, nb, 1));
 }
 
 }  // namespace kern

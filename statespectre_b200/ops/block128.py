@@ -208,12 +208,12 @@ def _forward(x, weight, bias, out_dtype, keep: bool):
         return (y.zero_() if bias is None else y.copy_(bias.expand_as(y))), quantize(x) if keep else None, wp
     C = native()
     work_bytes = C.linear_work_bytes(m, k)
+    pitch = -(-k // 16) * 16
     if keep:
         (q, scales), pitch = _empty_pair((m,), k, dev)
         work = torch.empty(work_bytes, dtype=torch.uint8, device=dev)
         ptrs = q.data_ptr(), pitch, scales.data_ptr(), work.data_ptr()
     else:
-        pitch = -(-k // 16) * 16
         work = torch.empty(work_bytes + m * pitch, dtype=torch.uint8, device=dev)
         ptrs = work.data_ptr() + work_bytes, pitch, 0, work.data_ptr()
     _launch(x.get_device(), C.k_linear_block128, x.data_ptr(), ldx, _TYPE[x.dtype], *ptrs, work_bytes, wq.data_ptr(),
