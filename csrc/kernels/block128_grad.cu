@@ -66,7 +66,7 @@ struct Config {
     // Tiles in flight. From its load to the end of its product a tile of A
     // lives about 3700 cycles, one of Q (until it is converted) 2500, a
     // converted one 2000; a step takes 512.
-    static constexpr uint32_t NA = 7, NQ = 5, NB = 4;
+    static constexpr uint32_t NA = 6, NQ = 6, NB = 4;
     static constexpr uint32_t off_q = NA * a_bytes, off_b = off_q + NQ * q_bytes, off_out = off_b + NB * b_bytes;
     static constexpr uint32_t out_bytes = 32 * 64;  // of one storing warp: 32 rows of 64 bytes
     static constexpr uint32_t off_scale = off_out + 4 * out_bytes;
@@ -76,6 +76,9 @@ struct Config {
     static constexpr uint32_t tmem_cols = 2 * BN;
     static_assert(smem <= 227 * 1024 && tmem_cols <= 512, "");
     static_assert(a_bytes % 1024 == 0 && q_bytes % 1024 == 0 && b_bytes % 1024 == 0 && out_bytes % 1024 == 0, "");
+    // A slot always belongs to one group of converters: a group that saw only
+    // some uses of a slot could take one phase of its barrier for another.
+    static_assert(NQ % kGroups == 0 && NB % kGroups == 0, "");
     static_assert(off_out >= kSide * BN * 4 || CG == 2, "the split reduction's tile");
 };
 
