@@ -14,8 +14,8 @@
 // then holds little but weights. Per 128 x BN tile and block the tensor core
 // takes 2 BN cycles and the epilogue's multiply-adds BN issue slots of each scheduler.
 //
-// Warps: 0 loads (TMA in the 128-byte swizzle), 1 and 3 issue the products, 2
-// owns the tensor memory, the rest are the epilogue.
+// Warps: 0 loads (TMA in the 128-byte swizzle), 1 issues the products, 2 owns
+// the tensor memory, 3 idles, the rest are the epilogue.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -61,7 +61,7 @@ struct Config {
     static constexpr uint32_t stage_bytes = w_bytes + x_bytes + sx_words * 4;
     static constexpr uint32_t stage_pitch = (stage_bytes + 1023) / 1024 * 1024;
     static constexpr uint32_t tmem_sx = NBUF * BN;             // factors of x: four columns for 128 tokens
-    static constexpr uint32_t tmem_sw = tmem_sx + 2 * sx_words / 32;  // two sets of them; factors of w: all 1
+    static constexpr uint32_t tmem_sw = tmem_sx + sx_words / 32;  // factors of w: all 1
     static constexpr uint32_t tmem_used = tmem_sw + 4;
     static constexpr uint32_t tmem_cols = tmem_used <= 64 ? 64 : tmem_used <= 128 ? 128 : tmem_used <= 256 ? 256 : 512;
     static constexpr uint32_t off_bar = ST * stage_pitch;
@@ -79,7 +79,6 @@ struct Config {
     static_assert(!SHIFT || 128 * kFew + 256 * kMany <= 384 * kEven, "a split that the block has registers for");
     static_assert(tmem_used <= 512 && tmem_cols * per_sm <= 512, "tensor memory");
     static_assert(smem * per_sm <= 227 * 1024, "shared memory");
-    static_assert(ST >= NBUF && NBUF >= 2, "the issuing warps' order of waits");
     static_assert(CPT % CH == 0 && BN % 16 == 0 && (CG == 1 || BN % 32 == 0), "");
     static_assert(x_bytes % 1024 == 0 && w_bytes % 1024 == 0, "operands start on the swizzle's 1024 bytes");
     // the split reduction keeps a 128 x BN fp32 tile in the stages
@@ -239,43 +238,38 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
             }
             __syncwarp();
         }
-        if ((warp == 1 || warp == 3) && half == 0) {
-            // Two warps issue, each every second block: waiting for a stage
-            // and a buffer, four products, the factors and two commits take
-            // one warp 600 cycles, where the products take 448.
+        if (warp == 1 && half == 0) {
             constexpr uint32_t idesc = instr_desc_mxf8(kLanes * C::CG, C::BN);
-            const uint32_t mine = warp / 2, sx = tmem + C::tmem_sx + mine * C::sx_words / 32;
             const bool leader = elect_one();
             uint32_t it = 0, s = 0, b = 0, sphase = 0, bphase = 1;
             bool ok = true;
             for (uint32_t t = first_tile; ok && t < tiles; t += step)
                 for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                    if ((it & 1) == mine) {
-                        // The buffer first: the epilogue frees them in order,
-                        // so all blocks up to NBUF back have been multiplied,
-                        // this stage's last one among them. Otherwise the
-                        // stage's barrier could be a phase behind, and the test
-                        // of its parity pass too early (this warp sees only
-                        // every second use of a stage).
-                        ok = mbar_wait<C::CG == 2>(tempty(b), bphase, guard, kWaitTmemEmpty) &&
-                             mbar_wait(full(s), sphase, guard, kWaitFull);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        tc_fence_after();
-                        if (leader) {
-                            const uint32_t src = base + s * C::stage_pitch, d = tmem + b * C::BN;
+                    // the factors go ahead of the wait for a buffer: copies and products run in order
+                    const uint32_t src = base + s * C::stage_pitch;
+                    ok = __all_sync(0xffffffffu, mbar_wait(full(s), sphase, guard, kWaitFull));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (leader) {
 #pragma unroll
-                            for (uint32_t i = 0; i < C::sx_words; i += 128)
-                                scales_to_tmem<C::CG>(sx + i / 32, src + C::w_bytes + C::x_bytes + i * 4);
-                            const uint64_t dw = operand_desc(src), dx = operand_desc(src + C::w_bytes);
-#pragma unroll
-                            for (uint32_t k = 0; k < 4; ++k)  // 32 values, 32 bytes, a step
-                                mma_mxf8<C::CG>(d, dw + 2 * k, dx + 2 * k, idesc, tmem + C::tmem_sw, sx, k > 0);
-                            mma_commit<C::CG>(empty(s));
-                            mma_commit<C::CG>(tfull(b));
-                        }
-                        __syncwarp();
+                        for (uint32_t i = 0; i < C::sx_words; i += 128)
+                            scales_to_tmem<C::CG>(tmem + C::tmem_sx + i / 32, src + C::w_bytes + C::x_bytes + i * 4);
                     }
+                    __syncwarp();
+                    ok = __all_sync(0xffffffffu, mbar_wait<C::CG == 2>(tempty(b), bphase, guard, kWaitTmemEmpty));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (leader) {
+                        const uint32_t d = tmem + b * C::BN;
+                        const uint64_t dw = operand_desc(src), dx = operand_desc(src + C::w_bytes);
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k)  // 32 values, 32 bytes, a step
+                            mma_mxf8<C::CG>(d, dw + 2 * k, dx + 2 * k, idesc, tmem + C::tmem_sw, tmem + C::tmem_sx,
+                                            k > 0);
+                        mma_commit<C::CG>(empty(s));
+                        mma_commit<C::CG>(tfull(b));
+                    }
+                    __syncwarp();
                     if (++s == C::ST) s = 0, sphase ^= 1;
                     if (++b == C::NBUF) b = 0, bphase ^= 1;
                 }
