@@ -79,7 +79,8 @@ struct Config {
     // A slot always belongs to one group of converters: a group that saw only
     // some uses of a slot could take one phase of its barrier for another.
     static_assert(NQ % kGroups == 0 && NB % kGroups == 0, "");
-    static_assert(off_out >= kSide * BN * 4 || CG == 2, "the split reduction's tile");
+    static constexpr uint32_t part_pitch = BN + 4;  // words of a row of partial sums: rows on different banks
+    static_assert(off_out >= kSide * part_pitch * 4, "the split reduction's tile");
 };
 
 // Position in a ring of N.
@@ -155,7 +156,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 3) tmem_alloc<C::CG>(base + C::off_misc, C::tmem_cols);
     tc_fence_before();
     __syncthreads();
-    if (C::CG == 2 || a.split > 1) cluster_sync();
+    if (C::CG == 2)
+        cluster_sync();
+    else if (a.split > 1)
+        cluster_arrive();  // waited for where the parts meet
     tc_fence_after();
     const uint32_t tmem = misc[0];
 
@@ -356,9 +360,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (share) {
                     // Partial sums meet in shared memory: the rings are free
                     // (the last product is done, one tile to a CTA).
+                    uint32_t* to = reinterpret_cast<uint32_t*>(sm) + my_lane * C::part_pitch + c;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        reinterpret_cast<uint32_t*>(sm)[(c + i) * kSide + my_lane] = v[i];
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<uint4*>(to + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                 } else if (row0 >= a.ni || j0 + c >= a.nj) {
                     // nothing of this piece is inside
                 } else if (a.tiled) {
@@ -396,11 +401,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                         __syncwarp();
                         if (lane == 0) tma_store(&map_out, base + stage, j0 + c, row0);
                     }
-                } else if (row0 + lane < a.ni) {
+                } else {
+                    // Rows that start anywhere: turned around in shared memory,
+                    // 16 columns at a time, so that lanes store neighbours.
+                    float* turn = reinterpret_cast<float*>(sm + stage);
 #pragma unroll
-                    for (uint32_t i = 0; i < 32; ++i)
-                        if (j0 + c + i < a.nj)
-                            store_one(a, int64_t(row0 + lane) * a.ld + j0 + c + i, __uint_as_float(v[i]));
+                    for (uint32_t p = 0; p < 2; ++p) {
+                        __syncwarp();
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) turn[i * 32 + (lane ^ i)] = __uint_as_float(v[16 * p + i]);
+                        __syncwarp();
+                        const uint32_t i = lane % 16, col = j0 + c + 16 * p + i;
+#pragma unroll 4
+                        for (uint32_t r = lane / 16; r < 32; r += 2)
+                            if (row0 + r < a.ni && col < a.nj)
+                                store_one(a, int64_t(row0 + r) * a.ld + col, turn[i * 32 + (r ^ i)]);
+                    }
                 }
                 __syncwarp();
             }
@@ -418,17 +434,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     if (C::CG == 1 && a.split > 1) {
         __syncthreads();
+        cluster_wait();
         cluster_sync();
         uint32_t i0, j0;
         place(first_tile, &i0, &j0);
         // every CTA of the cluster adds its share of the rows, in the order of the parts
         const uint32_t from = kSide * part / a.split, rows = kSide * (part + 1) / a.split - from;
-        for (uint32_t e = threadIdx.x; e < rows * C::BN; e += kThreads) {
-            const uint32_t r = from + e / C::BN, c = e % C::BN;
+        for (uint32_t e = threadIdx.x; e < rows * (C::BN / 4); e += kThreads) {
+            const uint32_t r = from + e / (C::BN / 4), c = e % (C::BN / 4) * 4;
             if (i0 + r >= a.ni || j0 + c >= a.nj) continue;
-            float sum = 0.f;
-            for (uint32_t p = 0; p < a.split; ++p) sum += ld_cluster(map_to_rank(base + (c * kSide + r) * 4, p));
-            store_one(a, int64_t(i0 + r) * a.ld + j0 + c, sum);
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            for (uint32_t p = 0; p < a.split; ++p) {
+                const float4 v = ld_cluster4(map_to_rank(base + (r * C::part_pitch + c) * 4, p));
+                sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+            }
+            const int64_t at = int64_t(i0 + r) * a.ld + j0 + c;
+            if (a.tiled && j0 + c + 4 <= a.nj) {  // four columns start on 8 or 16 bytes
+                if (a.type == 2)
+                    *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                else
+                    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
+                        make_uint2(pack16(a.type, sum[0], sum[1]), pack16(a.type, sum[2], sum[3]));
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+                    if (j0 + c + i < a.nj) store_one(a, at + i, sum[i]);
+            }
         }
     }
     tc_fence_before();
@@ -493,17 +524,20 @@ cudaError_t run(MatIn dy, int64_t dy_rows, int64_t dy_cols, const Block128In& q,
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-// Pairs of CTAs once their tiles fill the GPU, else single CTAs with the sum
-// in as many parts as there are SMs for, of two steps at least.
+// A step takes a pair and a single CTA the same 0.45 us, and a pair does four
+// times the work. So pairs, unless even the single CTAs' tiles leave half of
+// the SMs idle: then single CTAs, and the sum in as many parts (of at least
+// eight steps, under which joining them costs more than it saves) as there are
+// SMs for. Microseconds with pairs / single / the rule's split:
+//   32 single tiles x 224 steps  78 / 86 / 28 (4)     64 x 128  47 / 51 / 31 (2)
+//   40 x 80  33 / 34 / 19 (3)   40 x 2  8.3 / 6.6 / -   112 x 64  37 / 42 / -   320 x 32  29 / 41 / -
 template <bool A_T>
 cudaError_t choose(MatIn dy, int64_t dy_rows, int64_t dy_cols, const Block128In& q, MatOut out, FloatType type,
                    int64_t ni, int64_t nj, int64_t nt, cudaStream_t s) {
-    const int64_t sms = sm_count(), pairs = (ni + 255) / 256 * ((nj + 255) / 256);
-    if (pairs * 2 >= sms) return run<Config<A_T, 2>>(dy, dy_rows, dy_cols, q, out, type, ni, nj, nt, 1, s);
-    const int64_t tiles = (ni + 127) / 128 * ((nj + 127) / 128), steps = (nt + kStep - 1) / kStep;
-    uint32_t split = 1;
-    while (split < 8 && tiles * split * 2 <= sms && steps >= split * 4) split *= 2;
-    return run<Config<A_T, 1>>(dy, dy_rows, dy_cols, q, out, type, ni, nj, nt, split, s);
+    const int64_t sms = sm_count(), tiles = (ni + 127) / 128 * ((nj + 127) / 128), steps = (nt + kStep - 1) / kStep;
+    if (tiles * 2 > sms) return run<Config<A_T, 2>>(dy, dy_rows, dy_cols, q, out, type, ni, nj, nt, 1, s);
+    const int64_t split = std::max<int64_t>(1, std::min<int64_t>({8, sms / tiles, steps / 8}));
+    return run<Config<A_T, 1>>(dy, dy_rows, dy_cols, q, out, type, ni, nj, nt, uint32_t(split), s);
 }
 
 bool args_ok(const MatIn& dy, int64_t n, const Block128In& q, const MatOut& out, int64_t k, FloatType type) {

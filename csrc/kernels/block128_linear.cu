@@ -452,10 +452,13 @@ cudaError_t run(const Problem& p, uint32_t split) {
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-// Parts of the sum: enough to give every SM work, at least two blocks each.
-uint32_t parts(int64_t tiles, int64_t nb, int per_sm) {
+// Parts of the sum while they reach SMs that have nothing to do, of two blocks
+// at least: n = 5120 (40 tiles), one token, 1 / 2 / 4 / 8 parts 16.3 / 13.5 /
+// 12.7 / 16.6 us; n = 14336 (112 tiles), 16 tokens, 1 / 2 parts 16.7 / 18.6.
+uint32_t parts(int64_t tiles, int64_t nb, int64_t room) {
+    const int64_t sms = sm_count();
     uint32_t s = 1;
-    while (s < 8 && tiles * s * 2 <= int64_t(sm_count()) * per_sm && nb >= s * 4) s *= 2;
+    while (s < 8 && tiles * s * 4 < sms * 3 && tiles * s * 2 <= room && nb >= s * 4) s *= 2;
     return s;
 }
 
@@ -478,11 +481,24 @@ cudaError_t linear_block128(MatIn x, FloatType xtype, Block128Out kept, void* wo
         return cudaErrorInvalidValue;
     const Problem p{x, xtype, kept, static_cast<uint32_t*>(work), work_bytes, w, bias, y, type, m, n, k, s};
     const int64_t nb = (k + 127) / 128, nt = (n + 127) / 128;
-    if (m <= 16) return run<Config<16, 1, 4, 5, 4, 2>>(p, parts(nt, nb, 2));
-    if (m <= 32) return run<Config<32, 1, 4, 5, 4, 2>>(p, parts(nt, nb, 2));
-    if (m <= 64) return run<Config<64, 1, 8, 8, 4, 1>>(p, parts(nt, nb, 1));
-    if (((m + 223) / 224) * ((n + 255) / 256) >= 74) return run<Config<224, 2, 8, 6, 2, 1>>(p, 1);
-    return run<Config<128, 1, 8, 6, 3, 1>>(p, parts((m + 127) / 128 * nt, nb, 1));
+    // Few tokens: the fewest columns that hold them (the rest of the columns
+    // costs time too: 24 tokens x 5120 x 5120 take 14.5 us with 32 columns, 16.7
+    // with 64), two CTAs an SM where they fit.
+    const int64_t sms = sm_count();
+    if (m <= 16) return run<Config<16, 1, 4, 5, 4, 2>>(p, parts(nt, nb, sms * 2));
+    if (m <= 32) return run<Config<32, 1, 4, 5, 4, 2>>(p, parts(nt, nb, sms * 2));
+    if (m <= 64) {
+        const int64_t split = std::max<int64_t>(1, std::min<int64_t>({8, sms / nt, nb / 2}));
+        return run<Config<64, 1, 8, 8, 4, 1>>(p, uint32_t(split));
+    }
+    // Else by the number of rounds of tiles, of 224 x 256 for a pair of CTAs
+    // or 128 x 128 for each: a block of the sum takes a round 0.47 or 0.385 us.
+    // 1531 x 3456 x 5001: 36.1 us in pairs, 46.5 in 128s; 1024 x 4096 x 4096 37.0, 30.6.
+    const int64_t pairs = (m + 223) / 224 * ((n + 255) / 256), tiles = (m + 127) / 128 * nt;
+    const int64_t rounds2 = (pairs * 2 + sms - 1) / sms, rounds1 = (tiles + sms - 1) / sms;
+    if (rounds2 * 11 < rounds1 * 9) return run<Config<224, 2, 8, 6, 2, 1>>(p, 1);
+    // the parts of a 128 x 128 tile are 64 KiB each to join: not for two of them
+    return run<Config<128, 1, 8, 6, 3, 1>>(p, tiles * 4 <= sms ? parts(tiles, nb, sms) : 1);
 }
 
 }  // namespace kern

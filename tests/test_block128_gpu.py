@@ -157,7 +157,8 @@ def test_quantize_writes_nothing_beside_its_rows():
 
 SHAPES = [(1, 128, 1), (1, 5120, 640), (2, 128, 129), (3, 384, 255), (7, 1792, 1003), (16, 256, 512), (17, 4096, 136),
           (33, 128, 40), (64, 1024, 384), (65, 640, 1000), (128, 512, 256), (129, 256, 257), (200, 3456, 130),
-          (256, 384, 512), (300, 2048, 777), (513, 128, 1025), (640, 1280, 2048), (1531, 896, 5001), (2100, 384, 3333)]
+          (256, 384, 512), (300, 2048, 777), (513, 128, 1025), (640, 1280, 2048), (1531, 896, 5001), (2100, 384, 3333),
+          (40, 4096, 1000), (100, 2048, 200), (20, 14336, 1024), (12, 5120, 4100)]
 
 
 @pytest.mark.parametrize("m,k,n", SHAPES)
@@ -231,7 +232,7 @@ def test_linear_repeats_bit_for_bit():
 # ---- its gradients ------------------------------------------------------------------------------------------------
 
 GRAD_SHAPES = [(1, 8, 16), (1, 1, 1), (2, 128, 128), (77, 520, 1000), (3, 1003, 257), (128, 256, 384), (130, 72, 40),
-               (257, 264, 1001), (64, 2048, 128), (1000, 136, 520), (512, 512, 512), (2051, 130, 260)]
+               (257, 264, 1001), (64, 2048, 128), (1000, 136, 520), (512, 512, 512), (2051, 130, 260), (5, 4096, 300), (1030, 200, 130), (600, 1500, 1400)]
 
 
 @pytest.mark.parametrize("m,n,k", GRAD_SHAPES)
