@@ -34,6 +34,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from .. import ops
 from .._native import native
 from . import fabric
 
@@ -179,7 +180,24 @@ class RolloutWeights:
         if not isinstance(v, tuple):
             return v
         q, sc = v
+        if q.is_cuda and q.shape[-1] % 128 == 0:
+            return ops.dequantize((q, sc))
         return (q.float().view(-1, 128) * sc.view(-1, 1)).view(q.shape).to(torch.bfloat16)
+
+    def linear(self, x: torch.Tensor, name: str, bias: Optional[str] = None) -> torch.Tensor:
+        """``x @ w.T`` with the 2-D parameter ``name`` as it was pushed (plus the parameter ``bias``). A quantized
+        weight is multiplied in 8 bits (``ops.linear``: ``x`` is quantized too, the sums are fp32, and the result has
+        ``x``'s dtype); its rows must be multiples of 128 values, so that no scale spans two of them. Others go
+        through ``torch.nn.functional.linear``."""
+        w = self.get(name)
+        b = None if bias is None else self.get(bias)
+        if not isinstance(w, tuple):
+            return torch.nn.functional.linear(x, w, b)
+        q, sc = w
+        if q.dim() != 2 or q.shape[1] % 128:
+            raise ValueError(f"{name}: a quantized weight of shape {tuple(q.shape)} has scales that span rows; its "
+                             "rows must be multiples of 128 values in two dimensions")
+        return ops.linear(x, (q, sc), b)
 
     def content_hashes(self, names: Optional[Sequence[str]] = None, stream=None) -> Dict[str, Tuple[int, int]]:
         """ssh128 of the received bytes of bf16 entries (equal to the trainer's
