@@ -112,13 +112,18 @@ def _pair(p, what: str):
     return q, scales if scales.is_contiguous() else scales.contiguous(), rows, cols, ld
 
 
-def _empty_pair(lead, cols: int, dev: torch.device):
+def _empty_pair(like: torch.Tensor, lead, cols: int):
     """Uninitialised (q, scales) of [*lead, cols] values, and q's pitch."""
     pitch = -(-cols // 16) * 16
-    q = torch.empty((*lead, pitch), dtype=_FP8, device=dev)
+    q = like.new_empty((*lead, pitch), dtype=_FP8)
     if pitch != cols:
         q = q[..., :cols]
-    return (q, torch.empty((*lead, -(-cols // BLOCK)), dtype=torch.float32, device=dev)), pitch
+    return (q, like.new_empty((*lead, -(-cols // BLOCK)), dtype=torch.float32)), pitch
+
+
+def _empty_rows(like: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of `like`'s shape and type."""
+    return torch.empty_like(like) if like.is_contiguous() else like.new_empty(like.shape)
 
 
 def quantize(x: torch.Tensor) -> Block128:
@@ -132,7 +137,7 @@ def quantize(x: torch.Tensor) -> Block128:
     code = _type(x.dtype, "x")
     lead = x.shape[:-1]
     x, rows, cols, ld = _matrix(x, "x")
-    (q, scales), pitch = _empty_pair(lead, cols, x.device)
+    (q, scales), pitch = _empty_pair(x, lead, cols)
     _launch(x.get_device(), native().k_quantize_block128, x.data_ptr(), ld, code, q.data_ptr(), pitch,
             scales.data_ptr(), rows, cols)
     return q, scales
@@ -143,7 +148,7 @@ def dequantize(x: Block128, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor
     ``quantize`` made the pair)."""
     code = _type(dtype, "dtype")
     q, scales, rows, cols, ld = _pair(x, "x")
-    out = torch.empty(x[0].shape, dtype=dtype, device=q.device)
+    out = q.new_empty(x[0].shape, dtype=dtype)
     _launch(q.get_device(), native().k_dequantize_block128, q.data_ptr(), ld, scales.data_ptr(), out.data_ptr(), cols,
             code, rows, cols)
     return out
@@ -194,7 +199,6 @@ def _forward(x, weight, bias, out_dtype, keep: bool):
         raise ValueError(f"x has shape {tuple(x.shape)}, the weight {k} columns")
     lead = x.shape[:-1]
     x, m, _, ldx = _matrix(x, "x")
-    dev = x.device
     _same_device(x, wq, "weight")
     if bias is not None:
         _same_device(x, bias, "bias")
@@ -203,18 +207,18 @@ def _forward(x, weight, bias, out_dtype, keep: bool):
         if bias.dtype != out_dtype:
             raise ValueError(f"bias must be {out_dtype} like the result; got {bias.dtype}")
         bias = bias.contiguous()
-    y = torch.empty((*lead, n), dtype=out_dtype, device=dev)
+    y = x.new_empty((*lead, n), dtype=out_dtype)
     if k == 0:
         return (y.zero_() if bias is None else y.copy_(bias.expand_as(y))), quantize(x) if keep else None, wp
     C = native()
     work_bytes = C.linear_work_bytes(m, k)
     pitch = -(-k // 16) * 16
     if keep:
-        (q, scales), pitch = _empty_pair((m,), k, dev)
-        work = torch.empty(work_bytes, dtype=torch.uint8, device=dev)
+        (q, scales), pitch = _empty_pair(x, (m,), k)
+        work = x.new_empty(work_bytes, dtype=torch.uint8)
         ptrs = q.data_ptr(), pitch, scales.data_ptr(), work.data_ptr()
     else:
-        work = torch.empty(work_bytes + m * pitch, dtype=torch.uint8, device=dev)
+        work = x.new_empty(work_bytes + m * pitch, dtype=torch.uint8)
         ptrs = work.data_ptr() + work_bytes, pitch, 0, work.data_ptr()
     _launch(x.get_device(), C.k_linear_block128, x.data_ptr(), ldx, _TYPE[x.dtype], *ptrs, work_bytes, wq.data_ptr(),
             ldw, ws.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr(), n, _TYPE[out_dtype], m, n, k)
@@ -237,7 +241,7 @@ def linear_input_grad(dy: torch.Tensor, weight: Block128, out_dtype: torch.dtype
     (d, m, n, ldd), (q, scales, rows, k, ld) = _gradient(dy, weight, "weight")
     if rows != n or weight[0].dim() != 2:
         raise ValueError(f"dy has {n} columns, the weight shape {tuple(weight[0].shape)}")
-    dx = torch.empty((*dy.shape[:-1], k), dtype=out_dtype, device=d.device)
+    dx = d.new_empty((*dy.shape[:-1], k), dtype=out_dtype)
     if n == 0:
         return dx.zero_()
     _launch(d.get_device(), native().k_matmul_input_grad, d.data_ptr(), ldd, q.data_ptr(), ld, scales.data_ptr(),
@@ -252,7 +256,7 @@ def linear_weight_grad(dy: torch.Tensor, x: Block128, out_dtype: torch.dtype = t
     (d, m, n, ldd), (q, scales, rows, k, ld) = _gradient(dy, x, "x")
     if rows != m:
         raise ValueError(f"dy has {m} rows, x {rows}")
-    dw = torch.empty((n, k), dtype=out_dtype, device=d.device)
+    dw = d.new_empty((n, k), dtype=out_dtype)
     if m == 0:
         return dw.zero_()
     _launch(d.get_device(), native().k_matmul_weight_grad, d.data_ptr(), ldd, q.data_ptr(), ld, scales.data_ptr(),
@@ -296,12 +300,14 @@ def swiglu_forward(gate: torch.Tensor, up: torch.Tensor):
     if up.dtype != gate.dtype or up.shape != shape:
         raise ValueError(f"up ({tuple(up.shape)}, {up.dtype}) must match gate ({tuple(shape)}, {gate.dtype})")
     _same_device(gate, up, "up")
-    dev = gate.device
     g, rows, cols, ldg = _matrix(gate, "gate")
     u, _, _, ldu = _matrix(up, "up")
-    h = torch.empty(shape, dtype=gate.dtype, device=dev)
-    kg, pitch = _empty_pair(shape[:-1], cols, dev)
-    ku, _ = _empty_pair(shape[:-1], cols, dev)
+    h = _empty_rows(gate)
+    kg, pitch = _empty_pair(g, shape[:-1], cols)
+    if pitch == cols:
+        ku = torch.empty_like(kg[0]), torch.empty_like(kg[1])
+    else:
+        ku, _ = _empty_pair(g, shape[:-1], cols)
     _launch(g.get_device(), native().k_swiglu_forward, g.data_ptr(), ldg, u.data_ptr(), ldu, code, h.data_ptr(), cols,
             kg[0].data_ptr(), kg[1].data_ptr(), ku[0].data_ptr(), ku[1].data_ptr(), pitch, rows, cols)
     return h, (kg, ku)
@@ -322,8 +328,7 @@ def swiglu_backward(dh: torch.Tensor, kept) -> Tuple[torch.Tensor, torch.Tensor]
                          f"{tuple(kept[1][0].shape)}")
     _same_device(d, gq, "kept gate")
     _same_device(d, uq, "kept up")
-    dg = torch.empty(dh.shape, dtype=dh.dtype, device=d.device)
-    du = torch.empty(dh.shape, dtype=dh.dtype, device=d.device)
+    dg, du = _empty_rows(dh), _empty_rows(dh)
     _launch(d.get_device(), native().k_swiglu_backward, d.data_ptr(), ldd, code, gq.data_ptr(), ldg, gs.data_ptr(),
             uq.data_ptr(), ldu, us.data_ptr(), dg.data_ptr(), du.data_ptr(), cols, rows, cols)
     return dg, du

@@ -142,7 +142,7 @@ def test_quantize_borders_and_values_that_are_not_finite():
 
 def test_quantize_writes_nothing_beside_its_rows():
     x = randn((4, 1000), 3)
-    (q, s), pitch = ops.block128._empty_pair((4,), 1000, x.device)
+    (q, s), pitch = ops.block128._empty_pair(x, (4,), 1000)
     base = torch.full((6, pitch), 0x55, dtype=torch.uint8, device="cuda")
     scales = torch.full((6, 8), 7.0, device="cuda")
     ops.block128.native().k_quantize_block128(x.data_ptr(), 1000, 0, base[1:].data_ptr(), pitch, scales[1:].data_ptr(),
