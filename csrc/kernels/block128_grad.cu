@@ -43,8 +43,11 @@ constexpr uint32_t kStep = 64;   // of t
 // The tensor core's fp32 additions round towards zero, so their error grows
 // with their number: 8192 steps of t, 512 additions, leave a result of normal
 // values 3e-6 off, 70000 5e-5. Longer sums are taken in runs of 8192, which
-// the storing warps add up, rounding to nearest.
-constexpr uint32_t kRun = 8192 / kStep;
+// the storing warps add up in tensor memory, rounding to nearest. Results in
+// fp32 are taken in runs of 2048, 1e-6 off, each added to the output as it is
+// stored: one tile has one owner, which waits for a run's stores before it
+// sends the next, so the order of the additions never changes.
+constexpr uint32_t kRun = 8192 / kStep, kRunAdded = 2048 / kStep;
 constexpr uint32_t kGroups = 2, kGroupWarps = 4;  // of converters: a group takes every second step
 constexpr uint32_t kThreads = 512;
 
@@ -73,13 +76,14 @@ struct Config {
     // converted one 2000; a step takes 512.
     static constexpr uint32_t NA = 6, NQ = 6, NB = 4;
     static constexpr uint32_t off_q = NA * a_bytes, off_b = off_q + NQ * q_bytes, off_out = off_b + NB * b_bytes;
-    static constexpr uint32_t out_bytes = 32 * 64;  // of one storing warp: 32 rows of 64 bytes
-    static constexpr uint32_t off_scale = off_out + 4 * out_bytes;
+    static constexpr uint32_t out_bytes = 32 * 64;  // of one storing warp: 32 rows of 64 bytes, twice
+    static constexpr uint32_t off_scale = off_out + 4 * 2 * out_bytes;
     static constexpr uint32_t off_bar = off_scale + NQ * kStep * 4;
     static constexpr uint32_t off_misc = off_bar + (2 * (NA + NQ + NB) + 4) * 8;
     static constexpr uint32_t smem = off_misc + 16 + 1024;
     static constexpr uint32_t tmem_cols = 2 * BN;
     static_assert(smem <= 227 * 1024 && tmem_cols <= 512, "");
+    static_assert(off_out % (2 * out_bytes) == 0, "turns by one bit");
     static_assert(a_bytes % 1024 == 0 && q_bytes % 1024 == 0 && b_bytes % 1024 == 0 && out_bytes % 1024 == 0, "");
     // A slot always belongs to one group of converters: a group that saw only
     // some uses of a slot could take one phase of its barrier for another.
@@ -113,13 +117,19 @@ __device__ __forceinline__ void store_one(const Args& a, int64_t at, float v) {
     else
         static_cast<float*>(a.out)[at] = v;
 }
-// The buffers of tensor memory that take the sums in turn: both, or where a
-// sum has several runs the first, with the second for their total.
-struct Results {
-    uint32_t at = 0, phase = 0, count;
-    __device__ __forceinline__ explicit Results(uint32_t steps) : count(steps > kRun ? 1 : 2) {}
+// The runs of a part of the sum, and the buffers of tensor memory that take
+// them in turn: both, or where the runs are added up there, the first, with
+// the second for their total.
+struct Runs {
+    bool added, total;
+    uint32_t length, at = 0, phase = 0;
+    __device__ __forceinline__ Runs(const Args& a, uint32_t steps) {
+        added = a.type == 2 && a.tiled && a.split == 1;
+        length = added ? kRunAdded : kRun;
+        total = !added && steps > kRun;
+    }
     __device__ __forceinline__ void next() {
-        if (++at == count) at = 0, phase ^= 1;
+        if (++at == (total ? 1 : 2)) at = 0, phase ^= 1;
     }
 };
 
@@ -234,11 +244,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool leader = elect_one();
             Ring<C::NA> ra;
             Ring<C::NB> rb;
-            Results rt(t1 - t0);
+            Runs rt(a, t1 - t0);
             bool ok = true;
             for (uint32_t t = first_tile; ok && t < tiles; t += step) {
+                uint32_t in_run = 0;
                 for (uint32_t k = t0; k < t1; ++k, ra.next(), rb.next()) {
-                    const bool first = (k - t0) % kRun == 0, last = k + 1 == t1 || (k + 1 - t0) % kRun == 0;
+                    const bool first = in_run == 0, last = k + 1 == t1 || in_run + 1 == rt.length;
+                    in_run = last ? 0 : in_run + 1;
                     ok = (!first || mbar_wait<C::CG == 2>(tempty(rt.at), rt.phase ^ 1, guard, kWaitTmemEmpty)) &&
                          mbar_wait(a_full(ra.at), ra.phase, guard, kWaitAFull) &&
                          mbar_wait<C::CG == 2>(b_full(rb.at), rb.phase, guard, kWaitBFull);
@@ -355,9 +367,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp >= 4) {
         const uint32_t quad = warp % 4, my_lane = quad * 32 + lane;
-        const uint32_t stage = C::off_out + quad * C::out_bytes;
-        Results rt(t1 - t0);
-        const bool runs = rt.count == 1;
+        uint32_t stage = C::off_out + quad * 2 * C::out_bytes;  // the two take turns
+        Runs rt(a, t1 - t0);
         bool ok = true;
         auto release = [&] {
             tc_fence_before();
@@ -370,15 +381,99 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             rt.next();
         };
+        const uint32_t lanes = quad * 32 << 16;
+        const bool share = C::CG == 1 && a.split > 1;
         for (uint32_t t = first_tile; ok && t < tiles; t += step) {
             uint32_t i0, j0;
             place(t, &i0, &j0);
-            const uint32_t lanes = quad * 32 << 16;
-            for (uint32_t k = t0; ok && k < t1; k += kRun) {
+            const uint32_t row0 = i0 + quad * 32;
+            auto store = [&](uint32_t from, bool add) {
+                if (add && lane == 0) tma_store_wait();  // for the run before
+#pragma unroll 1
+                for (uint32_t c = 0; c < C::BN; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld(from + c, v);
+                    tmem_ld_keep(v);
+                    if (share) {
+                        // Partial sums meet in shared memory: the rings are free
+                        // (the last product is done, one tile to a CTA).
+                        uint32_t* to = reinterpret_cast<uint32_t*>(sm) + my_lane * C::part_pitch + c;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4*>(to + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                    } else if (row0 >= a.ni || j0 + c >= a.nj) {
+                        // nothing of this piece is inside
+                    } else if (a.tiled) {
+                        // Through shared memory (in the 64-byte swizzle) and out as
+                        // tiles: a lane's own stores would each touch a line of
+                        // their own, and hold up the converters' traffic.
+                        const uint32_t at = lane * 64, swz = lane / 2 % 4;
+                        if (a.type == 2) {
+#pragma unroll
+                            for (int p = 0; p < 2; ++p) {
+                                if (lane == 0) tma_store_wait_read();
+                                __syncwarp();
+#pragma unroll
+                                for (uint32_t i = 0; i < 4; ++i)
+                                    *reinterpret_cast<uint4*>(sm + stage + at + (i ^ swz) * 16) = make_uint4(
+                                        v[16 * p + 4 * i], v[16 * p + 4 * i + 1], v[16 * p + 4 * i + 2], v[16 * p + 4 * i + 3]);
+                                fence_async_smem();
+                                __syncwarp();
+                                if (lane == 0 && j0 + c + 16 * p < a.nj) {
+                                    if (add)
+                                        tma_add(&map_out, base + stage, j0 + c + 16 * p, row0);
+                                    else
+                                        tma_store(&map_out, base + stage, j0 + c + 16 * p, row0);
+                                }
+                                stage ^= C::out_bytes;
+                            }
+                        } else {
+                            if (lane == 0) tma_store_wait_read();
+                            __syncwarp();
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; ++i) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    w[k] = pack16(a.type, __uint_as_float(v[8 * i + 2 * k]),
+                                                  __uint_as_float(v[8 * i + 2 * k + 1]));
+                                *reinterpret_cast<uint4*>(sm + stage + at + (i ^ swz) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                            fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0) tma_store(&map_out, base + stage, j0 + c, row0);
+                            stage ^= C::out_bytes;
+                        }
+                    } else {
+                        // Rows that start anywhere: turned around in shared memory,
+                        // 16 columns at a time, so that lanes store neighbours.
+                        float* turn = reinterpret_cast<float*>(sm + stage);
+#pragma unroll
+                        for (uint32_t p = 0; p < 2; ++p) {
+                            __syncwarp();
+#pragma unroll
+                            for (uint32_t i = 0; i < 16; ++i) turn[i * 32 + (lane ^ i)] = __uint_as_float(v[16 * p + i]);
+                            __syncwarp();
+                            const uint32_t i = lane % 16, col = j0 + c + 16 * p + i;
+#pragma unroll 4
+                            for (uint32_t r = lane / 16; r < 32; r += 2)
+                                if (row0 + r < a.ni && col < a.nj)
+                                    store_one(a, int64_t(row0 + r) * a.ld + col, turn[i * 32 + (r ^ i)]);
+                        }
+                    }
+                    __syncwarp();
+                }
+            };
+            for (uint32_t k = t0; k < t1; k += rt.length) {
                 ok = __all_sync(0xffffffffu, mbar_wait(tfull(rt.at), rt.phase, guard, kWaitTmemFull));
                 __syncwarp();
-                if (!ok || !runs) break;
+                if (!ok) break;
                 tc_fence_after();
+                if (!rt.total) {
+                    store(tmem + rt.at * C::BN + lanes, k > t0);
+                    release();
+                    continue;
+                }
 #pragma unroll 1
                 for (uint32_t c = 0; c < C::BN; c += 32) {  // total = run, or total + run
                     uint32_t v[32];
@@ -400,79 +495,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 release();
             }
             if (!ok) break;
-            tc_fence_after();
-            const uint32_t from = tmem + (runs ? 1 : rt.at) * C::BN + lanes;
-            const uint32_t row0 = i0 + quad * 32;
-            const bool share = C::CG == 1 && a.split > 1;
-#pragma unroll 1
-            for (uint32_t c = 0; c < C::BN; c += 32) {
-                uint32_t v[32];
-                tmem_ld(from + c, v);
-                tmem_ld_keep(v);
-                if (share) {
-                    // Partial sums meet in shared memory: the rings are free
-                    // (the last product is done, one tile to a CTA).
-                    uint32_t* to = reinterpret_cast<uint32_t*>(sm) + my_lane * C::part_pitch + c;
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4*>(to + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                } else if (row0 >= a.ni || j0 + c >= a.nj) {
-                    // nothing of this piece is inside
-                } else if (a.tiled) {
-                    // Through shared memory (in the 64-byte swizzle) and out as
-                    // tiles: a lane's own stores would each touch a line of
-                    // their own, and hold up the converters' traffic.
-                    const uint32_t at = lane * 64, swz = lane / 2 % 4;
-                    if (a.type == 2) {
-#pragma unroll
-                        for (int p = 0; p < 2; ++p) {
-                            if (lane == 0) tma_store_wait_read();
-                            __syncwarp();
-#pragma unroll
-                            for (uint32_t i = 0; i < 4; ++i)
-                                *reinterpret_cast<uint4*>(sm + stage + at + (i ^ swz) * 16) = make_uint4(
-                                    v[16 * p + 4 * i], v[16 * p + 4 * i + 1], v[16 * p + 4 * i + 2], v[16 * p + 4 * i + 3]);
-                            fence_async_smem();
-                            __syncwarp();
-                            if (lane == 0 && j0 + c + 16 * p < a.nj)
-                                tma_store(&map_out, base + stage, j0 + c + 16 * p, row0);
-                        }
-                    } else {
-                        if (lane == 0) tma_store_wait_read();
-                        __syncwarp();
-#pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                w[k] = pack16(a.type, __uint_as_float(v[8 * i + 2 * k]),
-                                              __uint_as_float(v[8 * i + 2 * k + 1]));
-                            *reinterpret_cast<uint4*>(sm + stage + at + (i ^ swz) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                        fence_async_smem();
-                        __syncwarp();
-                        if (lane == 0) tma_store(&map_out, base + stage, j0 + c, row0);
-                    }
-                } else {
-                    // Rows that start anywhere: turned around in shared memory,
-                    // 16 columns at a time, so that lanes store neighbours.
-                    float* turn = reinterpret_cast<float*>(sm + stage);
-#pragma unroll
-                    for (uint32_t p = 0; p < 2; ++p) {
-                        __syncwarp();
-#pragma unroll
-                        for (uint32_t i = 0; i < 16; ++i) turn[i * 32 + (lane ^ i)] = __uint_as_float(v[16 * p + i]);
-                        __syncwarp();
-                        const uint32_t i = lane % 16, col = j0 + c + 16 * p + i;
-#pragma unroll 4
-                        for (uint32_t r = lane / 16; r < 32; r += 2)
-                            if (row0 + r < a.ni && col < a.nj)
-                                store_one(a, int64_t(row0 + r) * a.ld + col, turn[i * 32 + (r ^ i)]);
-                    }
-                }
-                __syncwarp();
+            if (rt.total) {
+                tc_fence_after();
+                store(tmem + C::BN + lanes, false);
             }
-            if (!runs) release();
         }
         if (lane == 0) tma_store_wait();
     }

@@ -119,8 +119,16 @@ __device__ __forceinline__ void tma_store(const CUtensorMap* m, uint32_t src, in
                  : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// This thread's stores have read their source, or are complete.
-__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+// The same, added to what is there (fp32, to nearest).
+__device__ __forceinline__ void tma_add(const CUtensorMap* m, uint32_t src, int32_t x, int32_t y) {
+    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(m),
+                 "r"(x), "r"(y), "r"(src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// All but the last of this thread's stores have read their source; all are
+// complete.
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // Four bytes, zeros when !valid.
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {

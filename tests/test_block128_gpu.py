@@ -250,19 +250,20 @@ def test_weight_grad(m, n, k, out):
     check_product(ops.linear_weight_grad(dy, x, out), dy.double().t(), values(x), out, m)
 
 
-@pytest.mark.parametrize("m,n,k", [(20000, 40, 200), (33000, 300, 520), (8192, 64, 128), (8193, 64, 128)])
+@pytest.mark.parametrize("m,n,k", [(20000, 40, 200), (33000, 300, 520), (8192, 64, 128), (8193, 64, 128),
+                                   (2049, 600, 3000), (20000, 40, 201)])
 def test_long_sums(m, n, k):
-    """The tensor core rounds its fp32 additions towards zero, one for each 16 products; in a run of 8192 products that
-    is at most 512 units of 2^-23 of the magnitudes' sum, and the runs are added to nearest."""
+    """The tensor core rounds its fp32 additions towards zero, one for each 16 products. They come in runs, of 2048
+    products where fp32 results can be stored as tiles and of 8192 elsewhere, and the runs are added to nearest: 128
+    (512) units of 2^-23 of the magnitudes' sum for a run, 16 within a step, half a one for each run."""
+    units = (128 + 16 + m / 4096 + 1 if k % 4 == 0 else 512 + 16 + m / 16384 + 1) * 2.0 ** -23 * 1.01
     dy, x = randn((m, n), 1, 1.0) + 1, ops.quantize(randn((m, k), 2) + 1)  # a mean, so that errors add up
-    got = ops.linear_weight_grad(dy, x, FP32).double()
     a, b = dy.double().t(), values(x)
-    assert bool(((got - a @ b).abs() <= (512 + 2 * 16 + m / 8192 + 1) * 2.0 ** -23 * (a.abs() @ b.abs())).all())
-    w = ops.quantize(randn((m, k), 3) + 1)
-    dyt = dy.t().contiguous()
-    got = ops.linear_input_grad(dyt, w, FP32).double()
-    b = values(w)
-    assert bool(((got - a @ b).abs() <= (512 + 2 * 16 + m / 8192 + 1) * 2.0 ** -23 * (a.abs() @ b.abs())).all())
+    got = ops.linear_weight_grad(dy, x, FP32)
+    assert bool(((got.double() - a @ b).abs() <= units * (a.abs() @ b.abs())).all())
+    assert torch.equal(ops.linear_weight_grad(dy, x, FP32), got)
+    got = ops.linear_input_grad(dy.t().contiguous(), x, FP32)
+    assert bool(((got.double() - a @ b).abs() <= units * (a.abs() @ b.abs())).all())
 
 
 def test_gradients_of_views_and_empty_shapes():
