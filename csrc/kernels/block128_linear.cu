@@ -10,9 +10,19 @@
 //
 // The rows of w lie on the 128 lanes of tensor memory, so that sw is one
 // register of each epilogue thread and the addition one multiply-add for a
-// result; the tokens lie on its BN columns. With few tokens the tile
-// then holds little but weights. Per 128 x BN tile and block the tensor core
-// takes 2 BN cycles and the epilogue's multiply-adds BN issue slots of each scheduler.
+// result; the tokens lie on its BN columns. With few tokens the tile then
+// holds little but weights.
+//
+// Many tokens: a pair of CTAs owns 256 x 224 results. A block of the sum takes
+// the tensor core 448 cycles and the epilogue 112 multiply-adds a lane, 224
+// issue slots of each scheduler. 4096 x 5120 x 27648: 530 us (2.2 PFLOP/s), 675
+// in a loop of seconds. A block takes about 800 cycles: the issuing warp needs
+// 600 of them (two in turn were no faster), the epilogue 620. At 1000 W the SMs
+// run at 1.6 GHz; without the epilogue's arithmetic they run at 1.48 GHz and
+// need 416 us, so the power cap would take most of what fewer cycles gave.
+// Few tokens: the bytes of w, in tiles of 128 rows x 16, 32 or 64 tokens, the
+// sum in parts over a cluster. 16 tokens x 4096 x 14336: 14.9 us (4 TB/s), one
+// token x 5120 x 5120: 10.2 us, of which 3 to 4 are starting and joining.
 //
 // Warps: 0 loads (TMA in the 128-byte swizzle), 1 issues the products, 2 owns
 // the tensor memory, 3 idles, the rest are the epilogue.
@@ -112,7 +122,8 @@ __device__ __forceinline__ void store_one(const Args& a, int64_t at, float v) {
 }
 // One lane's results: output `row` for tokens c0 and on.
 template <typename T, int N>
-__device__ __forceinline__ void store_column(const Args& a, uint32_t row, uint32_t c0, const float (&acc)[N], float add) {
+__device__ __forceinline__ void store_column(const Args& a, uint32_t row, uint32_t c0, const float (&acc)[N],
+                                             float add) {
     T* p = static_cast<T*>(a.out) + int64_t(c0) * a.ld + row;
     const uint32_t left = a.m > c0 ? a.m - c0 : 0;
 #pragma unroll
@@ -142,7 +153,8 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
     const uint32_t part = C::CG == 1 ? in_cluster : 0;  // which part of the sum
     const uint32_t group = C::CG == 2 ? 2 : a.split;
     const uint32_t first_tile = blockIdx.x / group, step = gridDim.x / group, tiles = a.tiles_n * a.tiles_m;
-    const uint32_t kb0 = uint32_t(uint64_t(a.nb) * part / a.split), kb1 = uint32_t(uint64_t(a.nb) * (part + 1) / a.split);
+    const uint32_t kb0 = uint32_t(uint64_t(a.nb) * part / a.split);
+    const uint32_t kb1 = uint32_t(uint64_t(a.nb) * (part + 1) / a.split);
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < C::ST; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
@@ -477,7 +489,8 @@ cudaError_t linear_block128(MatIn x, FloatType xtype, Block128Out kept, void* wo
         return cudaErrorInvalidValue;
     if (m == 0) return cudaSuccess;
     if (n == 0) return kept.scales ? quantize_block128(x, xtype, kept, m, k, s) : cudaSuccess;
-    if (!x.ptr || x.ld < k || int(xtype) < 0 || int(xtype) > 2 || !q_ok(w, k) || !y.ptr || y.ld < n || !work || (reinterpret_cast<uintptr_t>(work) & 15))
+    if (!x.ptr || x.ld < k || int(xtype) < 0 || int(xtype) > 2 || !q_ok(w, k) || !y.ptr || y.ld < n || !work ||
+        (reinterpret_cast<uintptr_t>(work) & 15))
         return cudaErrorInvalidValue;
     const Problem p{x, xtype, kept, static_cast<uint32_t*>(work), work_bytes, w, bias, y, type, m, n, k, s};
     const int64_t nb = (k + 127) / 128, nt = (n + 127) / 128;

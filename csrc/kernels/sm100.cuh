@@ -152,7 +152,9 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The two halves of a barrier of which only the order of events matters.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 // Waits for the kernel ahead in the stream, where this one was launched to
 // start before its end.
@@ -181,10 +183,12 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
 template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
     if (CG == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols)
+                     : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     } else {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(cols)
+                     : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
 }
@@ -250,7 +254,8 @@ __device__ __forceinline__ void mma_mxf8(uint32_t d, uint64_t a, uint64_t b, uin
 // groups of 32 lanes. Runs in order with this thread's products.
 template <int CG>
 __device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint32_t src) {
-    const uint64_t desc = uint64_t((src & 0x3ffff) >> 4) | uint64_t(1) << 16 | uint64_t(128 >> 4) << 32 | uint64_t(1) << 46;
+    const uint64_t desc =
+        uint64_t((src & 0x3ffff) >> 4) | uint64_t(1) << 16 | uint64_t(128 >> 4) << 32 | uint64_t(1) << 46;
     if (CG == 1)
         asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
     else
@@ -267,7 +272,8 @@ __device__ __forceinline__ void tmem_fill4(uint32_t addr, uint32_t v) {
 template <int CG>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     if (CG == 1)
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+                     : "memory");
     else
         asm volatile(
             "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(

@@ -13,6 +13,9 @@ ssh128, the library's choice of form), hash_onepass (the per-thread-load
 hash kernel), hash_stream (ssh128 through the K4 bulk-copy pipeline), verify (K3
 local vs second buffer), push / push_fp8 (K4 into a second buffer, raw or
 quantized; --peer 1 puts that buffer on cuda:1 so the stores cross NVLink).
+Operators on fp8 block-128 tensors (--shape M,N,K: tokens, outputs, inputs):
+linear, input_grad, weight_grad, swiglu (M x K, both passes), checkpoint (M x K
+saved and loaded).
 The case is larger than the 126 MB L2 so DRAM counters are meaningful; it
 holds about 2x --mb of device memory and --mb of pinned host memory.
 """
@@ -26,6 +29,48 @@ import torch
 from .._native import native
 
 
+def _operator(name: str, shape: str, iters: int) -> None:
+    from . import dequantize, linear, linear_input_grad, linear_weight_grad, quantize, swiglu_backward, swiglu_forward
+
+    m, n, k = (int(v) for v in shape.split(","))
+    dev = torch.device("cuda", 0)
+
+    def rand(rows, cols, std=1.0):
+        return (torch.randn(rows, cols, device=dev) * std).to(torch.bfloat16)
+
+    flops, moved = 2 * m * n * k, 0
+    if name == "linear":
+        x, w = rand(m, k), quantize(rand(n, k, 0.02))
+        run = lambda: linear(x, w)  # noqa: E731
+    elif name == "input_grad":
+        dy, w = rand(m, n), quantize(rand(n, k, 0.02))
+        run = lambda: linear_input_grad(dy, w)  # noqa: E731
+    elif name == "weight_grad":
+        dy, x = rand(m, n), quantize(rand(m, k))
+        run = lambda: linear_weight_grad(dy, x)  # noqa: E731
+    else:
+        flops, moved = 0, m * k * (16 if name == "swiglu" else 6)
+        gate, up, dh = rand(m, k), rand(m, k), rand(m, k)
+        if name == "swiglu":
+            run = lambda: swiglu_backward(dh, swiglu_forward(gate, up)[1])  # noqa: E731
+        else:
+            run = lambda: dequantize(quantize(gate))  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    ev0, ev1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    ev0.record()
+    for _ in range(iters):
+        run()
+    ev1.record()
+    torch.cuda.synchronize()
+    ms = ev0.elapsed_time(ev1) / iters
+    rate = f"{flops / ms / 1e9:.0f} TFLOP/s" if flops else f"{moved / ms / 1e6:.0f} GB/s"
+    print(f"{name} {m} x {n} x {k}: {ms * 1e3:.1f} us, {rate}")
+
+
+OPERATORS = ("linear", "input_grad", "weight_grad", "swiglu", "checkpoint")
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--kernel", required=True, choices=["evict", "restore", "restore_fp8", "hash", "hash_onepass",
@@ -33,7 +78,8 @@ def main():
                                                           "evict_z", "restore_z", "evict_bulk", "restore_bulk",
                                                           "evict_z_stage", "restore_z_stage", "zscan_f32",
                                                           "evict_zf32", "restore_zf32", "evict_zf32_stage",
-                                                          "restore_zf32_stage"])
+                                                          "restore_zf32_stage", *OPERATORS])
+    ap.add_argument("--shape", default="2048,4096,9472", help="operators: tokens, outputs, inputs")
     ap.add_argument("--mb", type=int, default=512)
     ap.add_argument("--iters", type=int, default=3)
     ap.add_argument("--ctas", type=int, default=0)
@@ -45,6 +91,9 @@ def main():
                     help="push: 1 = delta mode with the destination table cleared before each launch "
                          "(every chunk stored after its digest), 2 = delta mode with nothing changed")
     a = ap.parse_args()
+    if a.kernel in OPERATORS:
+        _operator(a.kernel, a.shape, a.iters)
+        return
     C = native()
     n = a.mb << 20
     dev = torch.device("cuda", 0)

@@ -232,7 +232,8 @@ def test_linear_repeats_bit_for_bit():
 # ---- its gradients ------------------------------------------------------------------------------------------------
 
 GRAD_SHAPES = [(1, 8, 16), (1, 1, 1), (2, 128, 128), (77, 520, 1000), (3, 1003, 257), (128, 256, 384), (130, 72, 40),
-               (257, 264, 1001), (64, 2048, 128), (1000, 136, 520), (512, 512, 512), (2051, 130, 260), (5, 4096, 300), (1030, 200, 130), (600, 1500, 1400)]
+               (257, 264, 1001), (64, 2048, 128), (1000, 136, 520), (512, 512, 512), (2051, 130, 260), (5, 4096, 300),
+               (1030, 200, 130), (600, 1500, 1400)]
 
 
 @pytest.mark.parametrize("m,n,k", GRAD_SHAPES)
