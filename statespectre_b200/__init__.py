@@ -6,7 +6,8 @@ Layers (bottom up):
   _wire                 Python mirror of the control-plane wire schema
   api                   offload_context / Off / handles / canonical keys
   _rollout              RolloutWeightClient (sealed-version pulls)
-  ops/                  kernel-level entry points on torch tensors
+  ops/                  operators on fp8 block-128 tensors (product, gradients, gated
+                        activation, 8-bit checkpoints), kernel profiling command
   parallel/             NVLink data plane: peer buffers, DP dedup, weight sync
   models/               shapes of the workloads (Llama-3-8B, Qwen2.5-32B, KV cache)
   utils/                timing, GPU clock sampling, config helpers
