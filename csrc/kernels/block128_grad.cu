@@ -431,6 +431,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (a.type == 2) {
 #pragma unroll
                             for (int p = 0; p < 2; ++p) {
+                                // nothing to send must not take a turn: the wait counts what was sent
+                                if (j0 + c + 16 * p >= a.nj) break;
                                 if (lane == 0) tma_store_wait_read();
                                 __syncwarp();
 #pragma unroll
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                    v[16 * p + 4 * i + 3]);
                                 fence_async_smem();
                                 __syncwarp();
-                                if (lane == 0 && j0 + c + 16 * p < a.nj) {
+                                if (lane == 0) {
                                     if (add)
                                         tma_add(&map_out, base + stage, j0 + c + 16 * p, row0);
                                     else

@@ -32,8 +32,8 @@ _TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 # The current stream and device as plain numbers: torch.cuda's functions build
 # objects, which at the smallest sizes takes longer than the kernels.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _type(dtype: torch.dtype, what: str) -> int:

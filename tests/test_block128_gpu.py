@@ -267,6 +267,16 @@ def test_long_sums(m, n, k):
     assert bool(((got.double() - a @ b).abs() <= units * (a.abs() @ b.abs())).all())
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 4737, 2924), (3, 2000, 1004), (130, 1111, 268)])
+def test_many_short_tiles_repeat(m, n, k):
+    """Tiles whose sum is a step or two keep the stores behind one another; the last columns of a row fill only the
+    first half of a stored piece."""
+    dy, x = randn((m, n), 1), ops.quantize(randn((m, k), 2))
+    want = ops.linear_weight_grad(dy, x, FP32)
+    check_product(want, dy.double().t(), values(x), FP32, m)
+    assert all(torch.equal(ops.linear_weight_grad(dy, x, FP32), want) for _ in range(100))
+
+
 def test_gradients_of_views_and_empty_shapes():
     dy, x = randn((60, 300), 1), ops.quantize(randn((60, 200), 2))
     w = ops.quantize(randn((300, 200), 3))
