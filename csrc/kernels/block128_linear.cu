@@ -244,7 +244,8 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
             }
             if (*guard.abort && half == 0 && leader) {  // let copies in flight land before the block retires
                 const long long t0 = clock64();
-                for (uint32_t i = it > C::ST ? it - C::ST : 0; i < it; ++i)
+                const uint32_t end = max(it, ahead);
+                for (uint32_t i = end > C::ST ? end - C::ST : 0; i < end; ++i)
                     while (!mbar_test(full(i % C::ST), i / C::ST & 1) && clock64() - t0 < kWaitCycles / 8) {
                     }
             }

@@ -203,21 +203,6 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 template <int CG>
-__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    if (CG == 1)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-            "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
-            : "memory");
-}
-template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
     if (CG == 1)
         asm volatile(
@@ -232,7 +217,7 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
             "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
             : "memory");
 }
-// The same with a factor for each row of A and of B (e8m0, one byte a row).
+// e4m3 operands, with a factor for each row of A and of B (e8m0, one byte a row).
 template <int CG>
 __device__ __forceinline__ void mma_mxf8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scale_a,
                                          uint32_t scale_b, bool add) {
@@ -338,7 +323,7 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t mn_stri
     return uint64_t((addr & 0x3ffff) >> 4) | uint64_t(mn_stride >> 4) << 16 | uint64_t(1024 >> 4) << 32 |
            uint64_t(1) << 46 | uint64_t(2) << 61;
 }
-// Instruction descriptor: fp32 accumulators. `fmt` 0 = e4m3 / f16, 1 = bf16.
+// Instruction descriptor of kind::f16: fp32 accumulators. `fmt` 0 = f16, 1 = bf16.
 __host__ __device__ constexpr uint32_t instr_desc(int m, int n, uint32_t fmt, bool a_mn, bool b_mn) {
     return 1u << 4 | fmt << 7 | fmt << 10 | uint32_t(a_mn) << 15 | uint32_t(b_mn) << 16 | uint32_t(n >> 3) << 17 |
            uint32_t(m >> 4) << 24;
