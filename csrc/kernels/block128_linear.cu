@@ -15,7 +15,7 @@
 //
 // Many tokens: a pair of CTAs owns 256 x 224 results. A block of the sum takes
 // the tensor core 448 cycles and the epilogue 112 multiply-adds a lane, 224
-// issue slots of each scheduler. 4096 x 5120 x 27648: 530 us (2.2 PFLOP/s), 675
+// issue slots of each scheduler. 4096 x 5120 x 27648: 530 us (2.2 PFLOP/s), 660
 // in a loop of seconds. A block takes about 800 cycles: the issuing warp needs
 // 600 of them (two in turn were no faster), the epilogue 620. At 1000 W the SMs
 // run at 1.6 GHz; without the epilogue's arithmetic they run at 1.48 GHz and
