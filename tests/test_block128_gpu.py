@@ -617,3 +617,41 @@ def test_backward_captured_and_replayed():
         g.replay()
         want = step()
         assert all(torch.equal(a, b) for a, b in zip(captured, want))
+
+
+def test_kept_activations_leave_the_gpu_between_the_passes(sock_path):
+    """What the forward pass keeps goes to pinned host memory through a session and comes back for the backward pass;
+    the gradients are the same bits."""
+    from statespectre_b200 import in_process_daemon, offload_context
+
+    m, h, f = 512, 1024, 1536
+    x, dy = randn((m, h), 1), randn((m, h), 2, 1e-2)
+    wu, wd = (randn(s, i, 0.05).requires_grad_() for i, s in ((3, (2 * f, h)), (4, (h, f))))
+
+    def step():
+        both = ops.linear(x, wu)
+        return torch.autograd.grad(ops.linear(ops.swiglu(both[:, :f], both[:, f:]), wd), (wu, wd), dy)
+
+    want = step()
+    d = in_process_daemon(socket=sock_path, arena_mb=256, drain_on_complete=False)
+    try:
+        with offload_context(daemon_addr=sock_path, device="cuda:0", rank=0) as off:
+            handles = []
+
+            def pack(t):
+                if t.dtype != FP8:
+                    return t
+                handles.append(off.copy(t, wait=True))
+                return handles[-1]
+
+            def unpack(k):
+                return k if isinstance(k, torch.Tensor) else k.restore()
+
+            with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+                got = step()
+            assert sum(k.nbytes for k in handles) >= m * (h + 3 * f)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            for k in handles:
+                k.discard()
+    finally:
+        d.stop()
