@@ -15,7 +15,7 @@
 //
 // Many tokens: a pair of CTAs owns 256 x 224 results. A block of the sum takes
 // the tensor core 448 cycles and the epilogue 112 multiply-adds a lane, 224
-// issue slots of each scheduler. 4096 x 5120 x 27648: 530 us (2.2 PFLOP/s), 660
+// issue slots of each scheduler. 4096 x 5120 x 27648: 526 us (2.2 PFLOP/s), 650
 // in a loop of seconds. A block takes about 800 cycles: the issuing warp needs
 // 600 of them (two in turn were no faster), the epilogue 620. At 1000 W the SMs
 // run at 1.6 GHz; without the epilogue's arithmetic they run at 1.48 GHz and
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
         if (C::SHIFT) regs_more<C::kMany>();
         const uint32_t quad = warp % 4, mine = (warp - 4) / 4 * C::CPT;  // lanes, first column
         const uint32_t my_lane = quad * 32 + lane;
-        uint32_t it = 0;
+        uint32_t b = 0, bphase = 0;
         bool ok = true;
         for (uint32_t t = first_tile; ok && t < tiles; t += step) {
             uint32_t n0, tm;
@@ -309,11 +309,9 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
             float acc[C::CPT];
 #pragma unroll
             for (int i = 0; i < C::CPT; ++i) acc[i] = 0.f;
-            for (uint32_t kb = kb0; kb < kb1; ++kb, ++it) {
-                const uint32_t b = it % C::NBUF;
+            for (uint32_t kb = kb0; kb < kb1; ++kb) {
                 const float scale = next;
-                if (kb + 1 < kb1) next = __ldg(sw + kb + 1);
-                ok = mbar_wait(tfull(b), it / C::NBUF & 1, guard, kWaitTmemFull);
+                ok = mbar_wait(tfull(b), bphase, guard, kWaitTmemFull);
                 ok = __all_sync(0xffffffffu, ok);
                 __syncwarp();
                 if (!ok) break;
@@ -323,6 +321,7 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                 uint32_t v[NC][C::CH];
 #pragma unroll
                 for (int c = 0; c < NC; ++c) tmem_ld(from + c * C::CH, v[c]);
+                if (kb + 1 < kb1) next = __ldg(sw + kb + 1);
                 tmem_ld_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -334,6 +333,7 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                 }
 #pragma unroll
                 for (int i = 0; i < C::CPT; ++i) add_scaled(acc[i], v[i / C::CH][i % C::CH], scale);
+                if (++b == C::NBUF) b = 0, bphase ^= 1;
             }
             if (C::CG == 1 && a.split > 1) {
                 // Partial sums meet in shared memory: the stages are free (the
