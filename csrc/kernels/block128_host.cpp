@@ -58,16 +58,27 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+void* driver_entry(const char* name) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const cudaError_t e = cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &q);
+    return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? p : nullptr;
+}
 EncodeTiled encode_tiled() {
-    static const EncodeTiled fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            p = nullptr;
-        return reinterpret_cast<EncodeTiled>(p);
-    }();
+    static const EncodeTiled fn = reinterpret_cast<EncodeTiled>(driver_entry("cuTensorMapEncodeTiled"));
     return fn;
+}
+
+// A driver call needs a current context. A thread gets one with its first call
+// to the runtime that needs it, and an autograd thread's or a user's own may
+// have made none yet: its results came from torch's cache of memory.
+cudaError_t bind_thread() {
+    static const auto current = reinterpret_cast<CUresult (*)(CUcontext*)>(driver_entry("cuCtxGetCurrent"));
+    CUcontext ctx = nullptr;
+    if (current && current(&ctx) == CUDA_SUCCESS && ctx) return cudaSuccess;
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    return e == cudaSuccess ? cudaSetDevice(dev) : e;
 }
 
 }  // namespace
@@ -76,6 +87,7 @@ cudaError_t tile_map(CUtensorMap* map, CUtensorMapDataType type, const void* ptr
                      int64_t pitch, uint32_t box_cols, uint32_t box_rows, int swizzle) {
     const EncodeTiled fn = encode_tiled();
     if (!fn) return cudaErrorNotSupported;
+    if (const cudaError_t e = bind_thread()) return e;
     const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
     const cuuint64_t strides[1] = {cuuint64_t(pitch)};
     const cuuint32_t box[2] = {box_cols, box_rows}, step[2] = {1, 1};
