@@ -58,12 +58,21 @@ uint64_t linear_work_bytes(int64_t m, int64_t k);
 cudaError_t linear_block128(MatIn x, FloatType xtype, Block128Out kept, void* work, uint64_t work_bytes, Block128In w,
                             const void* bias, MatOut y, FloatType type, int64_t m, int64_t n, int64_t k,
                             cudaStream_t s);
+// Device memory of a gradient's own for the call (the caller may free or reuse
+// it in stream order). Without it the result is the same, but powers of two as
+// scales are treated like any others, which takes 16-bit results twice the
+// time and fp32 ones three times.
+struct GradWork {
+    uint32_t* words = nullptr;
+    uint32_t count = 0;
+};
+uint32_t grad_work_words(int64_t ni, int64_t nj);  // for a result of ni x nj; 0 if it needs none
 // dx[m, k] = dy w, dy [m, n] bf16, w [n, k] block-128.
 cudaError_t matmul_input_grad(MatIn dy, Block128In w, MatOut dx, FloatType type, int64_t m, int64_t n, int64_t k,
-                              cudaStream_t s);
+                              GradWork work, cudaStream_t s);
 // dw[n, k] = dy^T x, dy [m, n] bf16, x [m, k] block-128.
 cudaError_t matmul_weight_grad(MatIn dy, Block128In x, MatOut dw, FloatType type, int64_t m, int64_t n, int64_t k,
-                               cudaStream_t s);
+                               GradWork work, cudaStream_t s);
 
 uint64_t block128_launch_count();
 

@@ -5,12 +5,24 @@
 // Both are out[i, j] = sum_t A(i, t) Q[t, j] s[t, j / 128]: the 8-bit operand
 // is stored with the summed index as its row, and its scale changes with the
 // row, so it cannot leave the sum. Converter warps bring each tile of Q from
-// 8 bits to bf16 in shared memory, times its scale (fp32 product, one rounding
-// to bf16; none when the scale is a power of two, as in everything that
-// quantize made), and the tensor core multiplies it with dy as it is
-// (tcgen05.mma kind::f16, fp32 accumulators in tensor memory). The converted
-// tile and, for the weight gradient, dy's are read "MN-major": their rows run
-// along the output, not along the sum, so nothing is transposed.
+// 8 bits to bf16 in shared memory, times its scale, and the tensor core
+// multiplies it with dy as it is (tcgen05.mma kind::f16, fp32 accumulators in
+// tensor memory). The converted tile and, for the weight gradient, dy's are
+// read "MN-major": their rows run along the output, not along the sum, so
+// nothing is transposed.
+//
+// A value times a power of two, as in everything that quantize made, is exact
+// in bf16. Any other scale leaves up to 28 bits, of which one bf16 rounding
+// would drop 20: the gradient would be 2.3e-3 off the exact one where rounding
+// it to bf16 costs 1.7e-3. So where there is such a scale, each tile of Q goes
+// to the tensor core in parts, each the bf16 rounding of what the parts before
+// left over: two (2^-16 of a value) for results in 16 bits, three (2^-24) for
+// fp32. 4096 x 4096 x 14336, bf16 results: 369 us with powers of two, 727 us
+// with other scales.
+//
+// Which of the two it is, is found on the device: a CTA with a tile of its own
+// looks at the scales that it will use; for pairs, which use each scale many
+// times, a kernel ahead reads them all once (2 us).
 //
 // A pair of CTAs owns 256 x 256 outputs; each loads 128 rows of A and 128
 // columns of Q for 64 steps of t, and converts its 8192 values while the
@@ -33,6 +45,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "block128.h"
 #include "block128_host.h"
@@ -70,6 +83,8 @@ enum : uint32_t {
     kWaitTmemFull
 };
 
+constexpr uint32_t kOddThreads = 256;
+
 struct Args {
     const float* scales;
     void* out;
@@ -78,6 +93,8 @@ struct Args {
     uint32_t tiles_i, tiles_j, split;
     int type;  // FloatType
     bool tiled;  // the output can be stored in tiles (16-byte rows)
+    const uint32_t* odd;  // pairs: words of k_odd, any of them not 0 where a scale is no power of two; null: assume so
+    uint32_t odd_words;
     uint32_t* error;
 };
 
@@ -103,8 +120,10 @@ struct Config {
     static_assert(off_out % (2 * out_bytes) == 0, "turns by one bit");
     static_assert(a_bytes % 1024 == 0 && q_bytes % 1024 == 0 && b_bytes % 1024 == 0 && out_bytes % 1024 == 0, "");
     // A slot always belongs to one group of converters: a group that saw only
-    // some uses of a slot could take one phase of its barrier for another.
+    // some uses of a slot could take one phase of its barrier for another. With
+    // several parts to a step that takes a ring for each group.
     static_assert(NQ % kGroups == 0 && NB % kGroups == 0, "");
+    static constexpr uint32_t NBG = NB / kGroups;
     static constexpr uint32_t part_pitch = BN + 4;  // words of a row of partial sums: rows on different banks
     static_assert(off_out >= kSide * part_pitch * 4, "the split reduction's tile");
 };
@@ -150,13 +169,76 @@ struct Runs {
     }
 };
 
+// A scale that is no power of two (or 0, or infinite).
+__device__ __forceinline__ bool is_odd(float s) { return (__float_as_uint(s) & 0x7fffffu) != 0; }
+
+// Whether any of `count` scales is odd, one word for each CTA.
+__global__ void __launch_bounds__(kOddThreads)
+    k_odd(const float* __restrict__ scales, uint64_t count, uint32_t* words) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    bool any = false;
+#pragma unroll 8
+    for (uint64_t i = blockIdx.x * kOddThreads + threadIdx.x; i < count; i += uint64_t(gridDim.x) * kOddThreads)
+        any |= is_odd(__ldg(scales + i));
+    any = __syncthreads_or(any);
+    if (threadIdx.x == 0) words[blockIdx.x] = any;
+}
+
+// bf16 of two values. What is too large becomes the largest finite value, so
+// that there is something left for the next part.
+__device__ __forceinline__ uint32_t pack_finite(float lo, float hi) {
+    uint32_t w;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+// Part AT of two values: the rounding of what AT parts have left over; the LAST one may be infinite.
+template <int AT, bool LAST>
+__device__ __forceinline__ uint32_t part2(float lo, float hi) {
+#pragma unroll
+    for (int i = 0; i < AT; ++i) {
+        const uint32_t w = pack_finite(lo, hi);
+        lo -= __uint_as_float(w << 16);
+        hi -= __uint_as_float(w & 0xffff0000u);
+    }
+    return LAST ? pack16(0, lo, hi) : pack_finite(lo, hi);
+}
 // Four e4m3 values times a scale, as bf16.
+template <int AT, bool LAST>
 __device__ __forceinline__ uint2 convert4(uint32_t w, float s) {
     const __half2 lo(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w & 0xffff), __NV_E4M3));
     const __half2 hi(__nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(w >> 16), __NV_E4M3));
     const float2 a = __half22float2(lo), b = __half22float2(hi);
-    return make_uint2(pack16(0, a.x * s, a.y * s), pack16(0, b.x * s, b.y * s));
+    return make_uint2(part2<AT, LAST>(a.x * s, a.y * s), part2<AT, LAST>(b.x * s, b.y * s));
 }
+template <int AT, bool LAST>
+__device__ __forceinline__ void convert16(uint4 w, float s, uint4* o) {
+    const uint2 c0 = convert4<AT, LAST>(w.x, s), c1 = convert4<AT, LAST>(w.y, s);
+    const uint2 c2 = convert4<AT, LAST>(w.z, s), c3 = convert4<AT, LAST>(w.w, s);
+    o[0] = make_uint4(c0.x, c0.y, c1.x, c1.y);
+    o[1] = make_uint4(c2.x, c2.y, c3.x, c3.y);
+}
+// Half a row, 64 columns: four chunks of 16 bytes of Q that become eight of
+// the operand, each at its place in the 128-byte swizzle. The two halves take
+// the chunks in different order, which keeps eight lanes on eight banks.
+struct HalfRow {
+    uint32_t h, swz;
+    __device__ __forceinline__ uint4 load(const uint8_t* q, uint32_t i) const {
+        return *reinterpret_cast<const uint4*>(q + (((i ^ 2 * h) + 4 * h) ^ swz) * 16);
+    }
+    __device__ __forceinline__ void store(uint8_t* d, uint32_t i, uint4 v) const {
+        *reinterpret_cast<uint4*>(d + ((i ^ 4 * h) ^ swz) * 16) = v;
+    }
+    template <int AT, bool LAST>
+    __device__ __forceinline__ void convert(const uint8_t* q, float s, uint8_t* d) const {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            uint4 o[2];
+            convert16<AT, LAST>(load(q, i), s, o);
+            store(d, 2 * i, o[0]);
+            store(d, 2 * i + 1, o[1]);
+        }
+    }
+};
 
 template <typename C>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -188,6 +270,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t0 = uint32_t(uint64_t(steps) * part / a.split);
     const uint32_t t1 = uint32_t(uint64_t(steps) * (part + 1) / a.split);
 
+    // Tiles in groups of 8 row tiles, those fastest: what is in flight shares
+    // its rows of A and columns of Q through L2.
+    auto place = [&](uint32_t t, uint32_t* i0, uint32_t* j0) {
+        const uint32_t per = 8 * a.tiles_j, g = t / per, first = g * 8, in = t - g * per;
+        const uint32_t wide = min(8u, a.tiles_i - first);
+        *i0 = (first + in % wide) * kSide * C::CG + half * kSide;  // this CTA's rows
+        *j0 = in / wide * C::BN;                                   // the tile's columns
+    };
+
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < C::NA; ++s) mbar_init(a_full(s), 1), mbar_init(a_empty(s), 1);
         // the load's thread, and each lane that fetches scales
@@ -198,8 +289,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         misc[1] = 0;
     }
     if (warp == 3) tmem_alloc<C::CG>(base + C::off_misc, C::tmem_cols);
+    bool odd = false;
+    if (C::CG == 1 && first_tile < tiles) {  // its one tile: a part of a column of scales
+        uint32_t i0, j0;
+        place(first_tile, &i0, &j0);
+#pragma unroll 4
+        for (uint32_t row = t0 * kStep + threadIdx.x; row < min(t1 * kStep, a.nt); row += kThreads)
+            odd |= is_odd(__ldg(a.scales + uint64_t(row) * a.nb + j0 / 128));
+    }
+    if (C::CG == 2) {
+        odd = !a.odd;
+        grid_wait();
+        if (threadIdx.x < a.odd_words) odd |= *reinterpret_cast<const volatile uint32_t*>(a.odd + threadIdx.x) != 0;
+    }
     tc_fence_before();
-    __syncthreads();
+    // one value for a warp, as for `warp` above: 688 us for 8192 x 4096 x 14336, else 780
+    odd = __shfl_sync(0xffffffffu, __syncthreads_or(odd), 0);
     if (C::CG == 2)
         cluster_sync();
     else if (a.split > 1)
@@ -207,14 +312,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = misc[0];
 
-    // Tiles in groups of 8 row tiles, those fastest: what is in flight shares
-    // its rows of A and columns of Q through L2.
-    auto place = [&](uint32_t t, uint32_t* i0, uint32_t* j0) {
-        const uint32_t per = 8 * a.tiles_j, g = t / per, first = g * 8, in = t - g * per;
-        const uint32_t wide = min(8u, a.tiles_i - first);
-        *i0 = (first + in % wide) * kSide * C::CG + half * kSide;  // this CTA's rows
-        *j0 = in / wide * C::BN;                                   // the tile's columns
-    };
+    // of a step's tile of Q, where there are several
+    const uint32_t parts = a.type == 2 ? 3 : 2;
 
     if (warp == 0) {
         const bool leader = elect_one();
@@ -256,41 +355,61 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (half == 0) {
+        auto issue = [&](auto in_parts) {
+            constexpr bool PARTS = decltype(in_parts)::value;
             constexpr uint32_t idesc = instr_desc(kSide * C::CG, C::BN, 1, C::A_T, true);
             // 16 steps of t: 32 bytes of a row, or 16 rows of 128 bytes
             constexpr uint32_t a_next = C::A_T ? 2048 >> 4 : 32 >> 4, b_next = 2048 >> 4;
             const bool leader = elect_one();
             Ring<C::NA> ra;
-            Ring<C::NB> rb;
+            Ring<PARTS ? C::NBG : C::NB> rb, rb_other;  // of the group whose turn it is, and of the other
+            uint32_t turn = 0;
             Runs rt(a, t1 - t0);
             bool ok = true;
             for (uint32_t t = first_tile; ok && t < tiles; t += step) {
                 uint32_t in_run = 0;
-                for (uint32_t k = t0; k < t1; ++k, ra.next(), rb.next()) {
+                for (uint32_t k = t0; k < t1; ++k, ra.next()) {
                     const bool first = in_run == 0, last = k + 1 == t1 || in_run + 1 == rt.length;
                     in_run = last ? 0 : in_run + 1;
                     ok = (!first || mbar_wait<C::CG == 2>(tempty(rt.at), rt.phase ^ 1, guard, kWaitTmemEmpty)) &&
-                         mbar_wait(a_full(ra.at), ra.phase, guard, kWaitAFull) &&
-                         mbar_wait<C::CG == 2>(b_full(rb.at), rb.phase, guard, kWaitBFull);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (leader) {
-                        const uint64_t da = operand_desc(base + ra.at * C::a_bytes, C::A_T ? C::a_bytes / 2 : 16);
-                        const uint64_t db = operand_desc(base + C::off_b + rb.at * C::b_bytes, C::b_bytes / 2);
+                         mbar_wait(a_full(ra.at), ra.phase, guard, kWaitAFull);
+#pragma unroll 1
+                    for (uint32_t p = 0; p < (PARTS ? parts : 1); ++p, rb.next()) {
+                        const uint32_t slot = PARTS ? rb.at * kGroups + turn : rb.at;
+                        ok = ok && mbar_wait<C::CG == 2>(b_full(slot), rb.phase, guard, kWaitBFull);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (leader) {
+                            const uint64_t da = operand_desc(base + ra.at * C::a_bytes, C::A_T ? C::a_bytes / 2 : 16);
+                            const uint64_t db = operand_desc(base + C::off_b + slot * C::b_bytes, C::b_bytes / 2);
 #pragma unroll
-                        for (uint32_t i = 0; i < kStep / 16; ++i)
-                            mma_f16<C::CG>(tmem + rt.at * C::BN, da + i * a_next, db + i * b_next, idesc,
-                                           !first || i > 0);
-                        mma_commit<C::CG>(a_empty(ra.at));
-                        mma_commit<C::CG>(b_empty(rb.at));
-                        if (last) mma_commit<C::CG>(tfull(rt.at));
+                            for (uint32_t i = 0; i < kStep / 16; ++i)
+                                mma_f16<C::CG>(tmem + rt.at * C::BN, da + i * a_next, db + i * b_next, idesc,
+                                               !first || p > 0 || i > 0);
+                            const bool whole = !PARTS || p + 1 == parts;
+                            if (whole) mma_commit<C::CG>(a_empty(ra.at));
+                            mma_commit<C::CG>(b_empty(slot));
+                            if (last && whole) mma_commit<C::CG>(tfull(rt.at));
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    if (!ok) break;
                     if (last) rt.next();
+                    if constexpr (PARTS) {
+                        const auto r = rb;
+                        rb = rb_other;
+                        rb_other = r;
+                        turn = (turn + 1) % kGroups;
+                    }
                 }
             }
+        };
+        if (half == 0) {
+            if (__builtin_expect(odd, 0))
+                issue(std::true_type{});
+            else
+                issue(std::false_type{});
         }
     } else if (warp == 2) {
         const bool leader = elect_one();
@@ -330,61 +449,85 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
     } else if (warp >= 8) {
         const uint32_t mine = (warp - 8) / kGroupWarps, id = threadIdx.x % (kGroupWarps * 32);
-        const uint32_t row = id / 2, h = id % 2, swz = row % 8;
-        Ring<C::NQ> rq;
-        Ring<C::NB> rb;
-        uint32_t turn = 0;
-        bool ok = true;
-        for (uint32_t t = first_tile; ok && t < tiles; t += step) {
-            for (uint32_t k = t0; k < t1; ++k, rq.next(), rb.next()) {
-                if (turn == mine) {
-                    ok = mbar_wait(q_full(rq.at), rq.phase, guard, kWaitQFull);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    // Half a row: 64 columns, four chunks of 16 bytes of Q that
-                    // become eight of the operand, each at its place in the
-                    // 128-byte swizzle. The two halves take the chunks in
-                    // different order, which keeps eight lanes on eight banks.
-                    const uint8_t* q = sm + C::off_q + rq.at * C::q_bytes + row * 128;
-                    uint8_t* d = sm + C::off_b + rb.at * C::b_bytes + h * (C::b_bytes / 2) + row * 128;
-                    const float f = reinterpret_cast<const float*>(sm + C::off_scale)[rq.at * kStep + row];
-                    uint4 w[4];
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i)
-                        w[i] = *reinterpret_cast<const uint4*>(q + (((i ^ 2 * h) + 4 * h) ^ swz) * 16);
-                    uint4 o[8];
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const uint2 c0 = convert4(w[i].x, f), c1 = convert4(w[i].y, f);
-                        const uint2 c2 = convert4(w[i].z, f), c3 = convert4(w[i].w, f);
-                        o[2 * i] = make_uint4(c0.x, c0.y, c1.x, c1.y);
-                        o[2 * i + 1] = make_uint4(c2.x, c2.y, c3.x, c3.y);
-                    }
-                    ok = mbar_wait(b_empty(rb.at), rb.phase ^ 1, guard, kWaitBEmpty);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    if (lane == 0) mbar_arrive(q_empty(rq.at));
-#pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i)
-                        *reinterpret_cast<uint4*>(d + ((i ^ 4 * h) ^ swz) * 16) = o[i];
-                    fence_async_smem();
-                    __syncwarp();
-                    // The tensor core of this SM reads what was written here,
-                    // from this SM's shared memory: the fence above has put it
-                    // there, and the arrival at the first CTA of a pair, where
-                    // the product is issued, only has to come after it. A
-                    // release to the cluster would also wait for this SM's
-                    // global memory, 1300 to 1900 cycles a step.
-                    if (lane == 0) {
-                        if (C::CG == 2)
-                            mbar_arrive_remote(map_to_rank(b_full(rb.at), 0));
-                        else
-                            mbar_arrive(b_full(rb.at));
-                    }
+        const uint32_t row = id / 2;
+        const HalfRow at{id % 2, row % 8};
+        auto convert = [&](auto in_parts) {
+            constexpr bool PARTS = decltype(in_parts)::value;
+            Ring<C::NQ> rq;
+            Ring<PARTS ? C::NBG : C::NB> rb;
+            uint32_t turn = 0;
+            bool ok = true;
+            auto slot = [&] { return PARTS ? rb.at * kGroups + mine : rb.at; };
+            auto room = [&] {
+                ok = mbar_wait(b_empty(slot()), rb.phase ^ 1, guard, kWaitBEmpty);
+                return ok = __all_sync(0xffffffffu, ok);
+            };
+            auto written = [&] {
+                fence_async_smem();
+                __syncwarp();
+                // The tensor core of this SM reads what was written here,
+                // from this SM's shared memory: the fence above has put it
+                // there, and the arrival at the first CTA of a pair, where
+                // the product is issued, only has to come after it. A
+                // release to the cluster would also wait for this SM's
+                // global memory, 1300 to 1900 cycles a step.
+                if (lane == 0) {
+                    if (C::CG == 2)
+                        mbar_arrive_remote(map_to_rank(b_full(slot()), 0));
+                    else
+                        mbar_arrive(b_full(slot()));
                 }
-                turn = turn + 1 == kGroups ? 0 : turn + 1;
+            };
+            for (uint32_t t = first_tile; ok && t < tiles; t += step) {
+                for (uint32_t k = t0; k < t1; ++k, rq.next()) {
+                    if (turn == mine) {
+                        ok = mbar_wait(q_full(rq.at), rq.phase, guard, kWaitQFull);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        const uint8_t* q = sm + C::off_q + rq.at * C::q_bytes + row * 128;
+                        const float f = reinterpret_cast<const float*>(sm + C::off_scale)[rq.at * kStep + row];
+                        auto to = [&] {
+                            return sm + C::off_b + slot() * C::b_bytes + at.h * (C::b_bytes / 2) + row * 128;
+                        };
+                        if constexpr (!PARTS) {  // converted before there is room for it
+                            uint4 w[4], o[8];
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; ++i) w[i] = at.load(q, i);
+#pragma unroll
+                            for (uint32_t i = 0; i < 4; ++i) convert16<0, true>(w[i], f, o + 2 * i);
+                            if (!room()) break;
+                            if (lane == 0) mbar_arrive(q_empty(rq.at));
+                            uint8_t* d = to();
+#pragma unroll
+                            for (uint32_t i = 0; i < 8; ++i) at.store(d, i, o[i]);
+                            written();
+                        } else {
+#pragma unroll 1
+                            for (uint32_t p = 0; p < parts; ++p, rb.next()) {
+                                if (!room()) break;
+                                if (p == 0)
+                                    at.convert<0, false>(q, f, to());
+                                else if (p + 1 < parts)
+                                    at.convert<1, false>(q, f, to());
+                                else if (p == 1)
+                                    at.convert<1, true>(q, f, to());
+                                else
+                                    at.convert<2, true>(q, f, to());
+                                written();
+                            }
+                            if (!ok) break;
+                            if (lane == 0) mbar_arrive(q_empty(rq.at));
+                        }
+                    }
+                    if constexpr (!PARTS) rb.next();
+                    turn = turn + 1 == kGroups ? 0 : turn + 1;
+                }
             }
-        }
+        };
+        if (__builtin_expect(odd, 0))
+            convert(std::true_type{});
+        else
+            convert(std::false_type{});
     } else if (warp >= 4) {
         const uint32_t quad = warp % 4, my_lane = quad * 32 + lane;
         uint32_t stage = C::off_out + quad * 2 * C::out_bytes;  // the two take turns
@@ -571,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <typename C>
 cudaError_t run(MatIn dy, int64_t dy_rows, int64_t dy_cols, const Block128In& q, MatOut out, FloatType type, int64_t ni,
-                int64_t nj, int64_t nt, uint32_t split, cudaStream_t s) {
+                int64_t nj, int64_t nt, uint32_t split, GradWork work, cudaStream_t s) {
     Args a{};
     cudaError_t e = error_word(&a.error);
     if (e == cudaSuccess) e = allow_smem(reinterpret_cast<const void*>(k_grad<C>), C::smem);
@@ -598,12 +741,18 @@ cudaError_t run(MatIn dy, int64_t dy_rows, int64_t dy_cols, const Block128In& q,
     a.nb = uint32_t((nj + 127) / 128);
     a.tiles_i = uint32_t((ni + kSide * C::CG - 1) / (kSide * C::CG));
     a.tiles_j = uint32_t((nj + C::BN - 1) / C::BN);
+    const uint64_t scales = uint64_t(a.nb) * a.nt;
+    if (C::CG == 2 && work.words && work.count) {
+        a.odd = work.words;
+        a.odd_words = uint32_t(std::min<uint64_t>(
+            {work.count, uint64_t(sm_count()), kThreads, (scales + kOddThreads - 1) / kOddThreads}));
+    }
     a.split = C::CG == 2 ? 1 : split;
     a.type = int(type);
     const uint64_t tiles = uint64_t(a.tiles_i) * a.tiles_j;
     if (tiles * a.split > 0x7fffffff) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = C::smem;
     cfg.stream = s;
@@ -615,8 +764,18 @@ cudaError_t run(MatIn dy, int64_t dy_rows, int64_t dy_cols, const Block128In& q,
         at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
         cfg.numAttrs = 1;
     }
+    if (a.odd) {  // starts while the scales are being read
+        at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
     const uint64_t units = a.split > 1 ? tiles : std::min<uint64_t>(tiles, uint64_t(sm_count()) / group);
     cfg.gridDim = dim3(uint32_t(units * group));
+    if (a.odd) {
+        k_odd<<<a.odd_words, kOddThreads, 0, s>>>(q.scales, scales, work.words);
+        g_block128_launches.fetch_add(1, std::memory_order_relaxed);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
     e = cudaLaunchKernelEx(&cfg, k_grad<C>, ma, mq, mo, a);
     g_block128_launches.fetch_add(1, std::memory_order_relaxed);
     return e != cudaSuccess ? e : cudaGetLastError();
@@ -629,13 +788,15 @@ cudaError_t run(MatIn dy, int64_t dy_rows, int64_t dy_cols, const Block128In& q,
 // SMs for. Microseconds with pairs / single / the rule's split:
 //   32 single tiles x 224 steps  78 / 86 / 28 (4)     64 x 128  47 / 51 / 31 (2)
 //   40 x 80  33 / 34 / 19 (3)   40 x 2  8.3 / 6.6 / -   112 x 64  37 / 42 / -   320 x 32  29 / 41 / -
+int64_t single_tiles(int64_t ni, int64_t nj) { return (ni + 127) / 128 * ((nj + 127) / 128); }
+bool in_pairs(int64_t ni, int64_t nj) { return single_tiles(ni, nj) * 2 > sm_count(); }
 template <bool A_T>
 cudaError_t choose(MatIn dy, int64_t dy_rows, int64_t dy_cols, const Block128In& q, MatOut out, FloatType type,
-                   int64_t ni, int64_t nj, int64_t nt, cudaStream_t s) {
-    const int64_t sms = sm_count(), tiles = (ni + 127) / 128 * ((nj + 127) / 128), steps = (nt + kStep - 1) / kStep;
-    if (tiles * 2 > sms) return run<Config<A_T, 2>>(dy, dy_rows, dy_cols, q, out, type, ni, nj, nt, 1, s);
+                   int64_t ni, int64_t nj, int64_t nt, GradWork work, cudaStream_t s) {
+    const int64_t sms = sm_count(), tiles = single_tiles(ni, nj), steps = (nt + kStep - 1) / kStep;
+    if (in_pairs(ni, nj)) return run<Config<A_T, 2>>(dy, dy_rows, dy_cols, q, out, type, ni, nj, nt, 1, work, s);
     const int64_t split = std::max<int64_t>(1, std::min<int64_t>({8, sms / tiles, steps / 8}));
-    return run<Config<A_T, 1>>(dy, dy_rows, dy_cols, q, out, type, ni, nj, nt, uint32_t(split), s);
+    return run<Config<A_T, 1>>(dy, dy_rows, dy_cols, q, out, type, ni, nj, nt, uint32_t(split), work, s);
 }
 
 bool args_ok(const MatIn& dy, int64_t n, const Block128In& q, const MatOut& out, int64_t k, FloatType type) {
@@ -643,6 +804,7 @@ bool args_ok(const MatIn& dy, int64_t n, const Block128In& q, const MatOut& out,
     return aligned(dy.ptr) && dy.ld >= n && dy.ld % 8 == 0 && aligned(q.q) && q.scales && q.ld % 16 == 0 &&
            q.ld >= k && out.ptr && out.ld >= k && int(type) >= 0 && int(type) <= 2;
 }
+bool work_ok(const GradWork& w) { return reinterpret_cast<uintptr_t>(w.words) % 4 == 0; }
 bool dims_ok(int64_t a, int64_t b, int64_t c) {
     const int64_t most = 0x7fffff00;
     return a >= 0 && b >= 0 && c >= 0 && a <= most && b <= most && c <= most;
@@ -650,20 +812,24 @@ bool dims_ok(int64_t a, int64_t b, int64_t c) {
 
 }  // namespace
 
+uint32_t grad_work_words(int64_t ni, int64_t nj) {
+    return ni > 0 && nj > 0 && in_pairs(ni, nj) ? uint32_t(sm_count()) : 0;
+}
+
 cudaError_t matmul_input_grad(MatIn dy, Block128In w, MatOut dx, FloatType type, int64_t m, int64_t n, int64_t k,
-                              cudaStream_t s) {
+                              GradWork work, cudaStream_t s) {
     if (!dims_ok(m, n, k) || n == 0) return cudaErrorInvalidValue;
     if (m == 0 || k == 0) return cudaSuccess;
-    if (!args_ok(dy, n, w, dx, k, type)) return cudaErrorInvalidValue;
-    return choose<false>(dy, m, n, w, dx, type, m, k, n, s);
+    if (!args_ok(dy, n, w, dx, k, type) || !work_ok(work)) return cudaErrorInvalidValue;
+    return choose<false>(dy, m, n, w, dx, type, m, k, n, work, s);
 }
 
 cudaError_t matmul_weight_grad(MatIn dy, Block128In x, MatOut dw, FloatType type, int64_t m, int64_t n, int64_t k,
-                               cudaStream_t s) {
+                               GradWork work, cudaStream_t s) {
     if (!dims_ok(m, n, k) || m == 0) return cudaErrorInvalidValue;
     if (n == 0 || k == 0) return cudaSuccess;
-    if (!args_ok(dy, n, x, dw, k, type)) return cudaErrorInvalidValue;
-    return choose<true>(dy, m, n, x, dw, type, n, k, m, s);
+    if (!args_ok(dy, n, x, dw, k, type) || !work_ok(work)) return cudaErrorInvalidValue;
+    return choose<true>(dy, m, n, x, dw, type, n, k, m, work, s);
 }
 
 }  // namespace kern

@@ -70,16 +70,21 @@ void bind_block128(py::module_& m) {
                                       FloatType(type), mm, n, k, stream(s)),
                       "linear_block128");
     });
+    m.def("grad_work_words", &grad_work_words);
     m.def("k_matmul_input_grad", [](uint64_t dy, int64_t lddy, uint64_t wq, int64_t ldw, uint64_t ws, uint64_t dx,
-                                    int64_t lddx, int type, int64_t mm, int64_t n, int64_t k, uint64_t s) {
+                                    int64_t lddx, int type, int64_t mm, int64_t n, int64_t k, uint64_t s,
+                                    uint64_t work, uint32_t words) {
         check_product(matmul_input_grad(in(dy, lddy), qin(wq, ldw, ws), out(dx, lddx), FloatType(type), mm, n, k,
-                                        stream(s)),
-              "matmul_input_grad");
-    });
+                                        {reinterpret_cast<uint32_t*>(work), words}, stream(s)),
+                      "matmul_input_grad");
+    }, py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(),
+       py::arg(), py::arg(), py::arg("work") = 0, py::arg("words") = 0);
     m.def("k_matmul_weight_grad", [](uint64_t dy, int64_t lddy, uint64_t xq, int64_t ldx, uint64_t xs, uint64_t dw,
-                                     int64_t lddw, int type, int64_t mm, int64_t n, int64_t k, uint64_t s) {
+                                     int64_t lddw, int type, int64_t mm, int64_t n, int64_t k, uint64_t s,
+                                     uint64_t work, uint32_t words) {
         check_product(matmul_weight_grad(in(dy, lddy), qin(xq, ldx, xs), out(dw, lddw), FloatType(type), mm, n, k,
-                                         stream(s)),
-              "matmul_weight_grad");
-    });
+                                         {reinterpret_cast<uint32_t*>(work), words}, stream(s)),
+                      "matmul_weight_grad");
+    }, py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(), py::arg(),
+       py::arg(), py::arg(), py::arg("work") = 0, py::arg("words") = 0);
 }

@@ -234,9 +234,22 @@ def _gradient(dy: torch.Tensor, other: Block128, what: str):
     return _tiled(dy, "dy"), p
 
 
+def _launch_grad(fn, d, ldd, q, ld, scales, out, code, m, n, k, out_rows) -> None:
+    device = d.get_device()
+    if device == _current_device():
+        words = native().grad_work_words(out_rows, k)
+        work = d.new_empty(words, dtype=torch.int32) if words else None
+        fn(d.data_ptr(), ldd, q.data_ptr(), ld, scales.data_ptr(), out.data_ptr(), k, code, m, n, k,
+           _raw_stream(device), work.data_ptr() if words else 0, words)
+    else:
+        with torch.cuda.device(device):
+            _launch_grad(fn, d, ldd, q, ld, scales, out, code, m, n, k, out_rows)
+
+
 def linear_input_grad(dy: torch.Tensor, weight: Block128, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """``dy @ w`` for ``dy`` [..., n] (bfloat16) and a pair ``weight`` [n, k]: [..., k]. Each weight is brought to
-    bfloat16 for the tensor cores, exactly when its scale is a power of two; sums are in fp32."""
+    """``dy @ w`` for ``dy`` [..., n] (bfloat16) and a pair ``weight`` [n, k]: [..., k]. Each weight goes to the tensor
+    cores exactly where its scale is a power of two, else within 2^-16 of it (2^-24 for an fp32 result), which takes
+    two (three) products instead of one; sums are in fp32."""
     code = _type(out_dtype, "out_dtype")
     (d, m, n, ldd), (q, scales, rows, k, ld) = _gradient(dy, weight, "weight")
     if rows != n or weight[0].dim() != 2:
@@ -244,14 +257,14 @@ def linear_input_grad(dy: torch.Tensor, weight: Block128, out_dtype: torch.dtype
     dx = d.new_empty((*dy.shape[:-1], k), dtype=out_dtype)
     if n == 0:
         return dx.zero_()
-    _launch(d.get_device(), native().k_matmul_input_grad, d.data_ptr(), ldd, q.data_ptr(), ld, scales.data_ptr(),
-            dx.data_ptr(), k, code, m, n, k)
+    _launch_grad(native().k_matmul_input_grad, d, ldd, q, ld, scales, dx, code, m, n, k, m)
     return dx
 
 
 def linear_weight_grad(dy: torch.Tensor, x: Block128, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``dy.T @ x`` for ``dy`` [..., n] (bfloat16) and the kept pair ``x`` [..., k]: [n, k], summed over all rows in
-    fp32. The kept values go to the tensor cores as bfloat16, exactly when their scales are powers of two."""
+    fp32. The kept values go to the tensor cores exactly where their scales are powers of two, as ``quantize`` makes
+    them, else as in ``linear_input_grad``."""
     code = _type(out_dtype, "out_dtype")
     (d, m, n, ldd), (q, scales, rows, k, ld) = _gradient(dy, x, "x")
     if rows != m:
@@ -259,8 +272,7 @@ def linear_weight_grad(dy: torch.Tensor, x: Block128, out_dtype: torch.dtype = t
     dw = d.new_empty((n, k), dtype=out_dtype)
     if m == 0:
         return dw.zero_()
-    _launch(d.get_device(), native().k_matmul_weight_grad, d.data_ptr(), ldd, q.data_ptr(), ld, scales.data_ptr(),
-            dw.data_ptr(), k, code, m, n, k)
+    _launch_grad(native().k_matmul_weight_grad, d, ldd, q, ld, scales, dw, code, m, n, k, n)
     return dw
 
 
