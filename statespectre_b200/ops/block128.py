@@ -1,9 +1,11 @@
 """Operators on fp8 block-128 tensors.
 
-A block-128 tensor is the pair ``(q, scales)`` that ``handle.restore(cast="fp8_block128")`` and
-``RolloutWeights.get`` return: ``q`` holds e4m3 values, ``scales`` one fp32 factor for each 128 consecutive
-values of a row, and the pair stands for ``q * scale``. A row whose length is no multiple of 128 ends in a
-shorter block of its own, and rows of ``q`` start on 16-byte boundaries (a pair laid out otherwise is copied).
+A block-128 tensor is the pair ``(q, scales)`` that ``quantize`` makes: ``q`` holds e4m3 values, ``scales`` one
+fp32 factor for each 128 consecutive values of a row, [..., ceil(cols / 128)], and the pair stands for
+``q * scale``. A row whose length is no multiple of 128 ends in a shorter block of its own, and rows of ``q``
+start on 16-byte boundaries (a pair laid out otherwise is copied). ``handle.restore(cast="fp8_block128")`` and
+``RolloutWeights.get`` return the same with flat scales where rows are multiples of 128 values; for other widths
+their blocks run on from row to row, and the operators refuse the pair.
 
 * ``quantize`` / ``dequantize``: an activation to 8 bits and back, with power-of-two scales
 * ``linear``: ``x @ w.T`` on the fp8 tensor cores; with gradients, the quantised operands of the forward
@@ -106,9 +108,13 @@ def _pair(p, what: str):
         raise ValueError(f"{what}: scales must be float32; got {scales.dtype}")
     _same_device(q, scales, what)
     q, rows, cols, ld = _tiled(q, what)
-    if scales.numel() != rows * -(-cols // BLOCK):
+    blocks = -(-cols // BLOCK)
+    count = scales.numel()
+    last = scales.shape[-1] if scales.dim() else 0
+    # Flat scales (count == last) count on from one row to the next, which is the same where rows end on a block.
+    if count != rows * blocks or (count and last != blocks and (count != last or (rows > 1 and cols % BLOCK))):
         raise ValueError(f"{what}: {tuple(scales.shape)} scales do not fit {rows} rows of {cols} values: one for "
-                         f"each {BLOCK} values of a row")
+                         f"each {BLOCK} values of a row, flat only where rows are multiples of {BLOCK}")
     return q, scales if scales.is_contiguous() else scales.contiguous(), rows, cols, ld
 
 
