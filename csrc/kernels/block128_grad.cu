@@ -62,12 +62,13 @@ constexpr uint32_t kSide = 128;  // rows of A and columns of Q of one CTA
 constexpr uint32_t kStep = 64;   // of t
 // The tensor core's fp32 additions round towards zero, so their error grows
 // with their number: 8192 steps of t, 512 additions, leave a result of normal
-// values 3e-6 off, 70000 5e-5. Longer sums are taken in runs of 8192, which
-// the storing warps add up in tensor memory, rounding to nearest. Results in
-// fp32 are taken in runs of 2048, 1e-6 off, each added to the output as it is
-// stored: one tile has one owner, which waits for a run's stores before it
-// sends the next, so the order of the additions never changes.
-constexpr uint32_t kRun = 8192 / kStep, kRunAdded = 2048 / kStep;
+// values 3e-6 off, 70000 5e-5. Longer sums are taken in runs of 8192 terms,
+// 2048 for results in fp32 (1e-6 off; terms in three parts 640). The storing
+// warps add the runs up in tensor memory, rounding to nearest. In fp32 they
+// add each to the output as it is stored, if it can be stored in tiles and the
+// sum is not split: one tile has one owner, which waits for a run's stores
+// before it sends the next, so the order of the additions never changes.
+constexpr uint32_t kRun = 8192 / kStep, kRunFp32 = 2048 / kStep;
 constexpr uint32_t kGroups = 2, kGroupWarps = 4;  // of converters: a group takes every second step
 constexpr uint32_t kThreads = 512;
 
@@ -159,10 +160,10 @@ __device__ __forceinline__ void store_one(const Args& a, int64_t at, float v) {
 struct Runs {
     bool added, total;
     uint32_t length, at = 0, phase = 0;
-    __device__ __forceinline__ Runs(const Args& a, uint32_t steps) {
+    __device__ __forceinline__ Runs(const Args& a, uint32_t steps, uint32_t parts) {
         added = a.type == 2 && a.tiled && a.split == 1;
-        length = added ? kRunAdded : kRun;
-        total = !added && steps > kRun;
+        length = a.type == 2 ? kRunFp32 / parts : kRun;
+        total = !added && steps > length;
     }
     __device__ __forceinline__ void next() {
         if (++at == (total ? 1 : 2)) at = 0, phase ^= 1;
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             Ring<C::NA> ra;
             Ring<PARTS ? C::NBG : C::NB> rb, rb_other;  // of the group whose turn it is, and of the other
             uint32_t turn = 0;
-            Runs rt(a, t1 - t0);
+            Runs rt(a, t1 - t0, PARTS ? parts : 1);
             bool ok = true;
             for (uint32_t t = first_tile; ok && t < tiles; t += step) {
                 uint32_t in_run = 0;
@@ -531,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp >= 4) {
         const uint32_t quad = warp % 4, my_lane = quad * 32 + lane;
         uint32_t stage = C::off_out + quad * 2 * C::out_bytes;  // the two take turns
-        Runs rt(a, t1 - t0);
+        Runs rt(a, t1 - t0, odd ? parts : 1);
         bool ok = true;
         auto release = [&] {
             tc_fence_before();
