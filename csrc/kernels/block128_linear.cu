@@ -8,6 +8,13 @@
 // values) goes to one of several buffers of tensor memory, and the epilogue
 // warps add sw P_b to fp32 registers while the next block's product runs.
 //
+// A P_b can be far larger than what it adds to y, since the weight's scale is
+// not in it: activations of 2^128 times 448, 128 of them, would overflow. So
+// the factor of all weights is 2^-16 and not 1, which keeps every P_b in range
+// (subnormal ones lose nothing: the tensor core keeps them), and the sum gets
+// 2^16 back as it is stored. Results under 2^-110 give bits for that. (2^16 in
+// sw instead, with a way out for scales over 2^111, took 5 % more time.)
+//
 // The rows of w lie on the 128 lanes of tensor memory, so that sw is one
 // register of each epilogue thread and the addition one multiply-add for a
 // result; the tokens lie on its BN columns. With few tokens the tile then
@@ -44,6 +51,8 @@ namespace {
 using namespace sm100;
 
 constexpr uint32_t kLanes = 128, kBlock = 128;
+constexpr uint32_t kDown = 0x6f6f6f6fu;  // e8m0 of 2^-16
+constexpr float kUp = 65536.f;
 
 // Codes of waits that ran out.
 enum : uint32_t { kWaitEmpty = 101, kWaitFull, kWaitTmemEmpty, kWaitTmemFull };
@@ -71,7 +80,7 @@ struct Config {
     static constexpr uint32_t stage_bytes = w_bytes + x_bytes + sx_words * 4;
     static constexpr uint32_t stage_pitch = (stage_bytes + 1023) / 1024 * 1024;
     static constexpr uint32_t tmem_sx = NBUF * BN;             // factors of x: four columns for 128 tokens
-    static constexpr uint32_t tmem_sw = tmem_sx + sx_words / 32;  // factors of w: all 1
+    static constexpr uint32_t tmem_sw = tmem_sx + sx_words / 32;  // factors of w: all 2^-16
     static constexpr uint32_t tmem_used = tmem_sw + 4;
     static constexpr uint32_t tmem_cols = tmem_used <= 64 ? 64 : tmem_used <= 128 ? 128 : tmem_used <= 256 ? 256 : 512;
     static constexpr uint32_t off_bar = ST * stage_pitch;
@@ -128,7 +137,7 @@ __device__ __forceinline__ void store_column(const Args& a, uint32_t row, uint32
     const uint32_t left = a.m > c0 ? a.m - c0 : 0;
 #pragma unroll
     for (int i = 0; i < N; ++i, p += a.ld)
-        if (uint32_t(i) < left) *p = rounded<T>(acc[i] + add);
+        if (uint32_t(i) < left) *p = rounded<T>(fmaf(acc[i], kUp, add));
 }
 
 template <typename C>
@@ -167,7 +176,7 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = misc[0];
-    if (warp >= 4 && warp < 8) tmem_fill4(tmem + C::tmem_sw + (warp % 4 * 32 << 16), 0x7f7f7f7fu);  // e8m0 of 1
+    if (warp >= 4 && warp < 8) tmem_fill4(tmem + C::tmem_sw + (warp % 4 * 32 << 16), kDown);
     tc_fence_before();
     __syncthreads();
     if (C::CG == 2)
@@ -377,8 +386,7 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
             if (row >= a.n || c >= a.m) continue;
             float sum = 0.f;
             for (uint32_t r = 0; r < a.split; ++r) sum += ld_cluster(map_to_rank(base + e * 4, r));
-            if (a.bias) sum += bias_at(a, row);
-            store_one(a, int64_t(c) * a.ld + row, sum);
+            store_one(a, int64_t(c) * a.ld + row, fmaf(sum, kUp, a.bias ? bias_at(a, row) : 0.f));
         }
     }
     tc_fence_before();
