@@ -21,6 +21,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from .._native import native
 
@@ -48,6 +49,8 @@ def _type(dtype: torch.dtype, what: str) -> int:
 def _on_gpu(t, what: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} must be a tensor; got {type(t).__name__}")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{what} has a tangent, and the operators have no forward-mode derivatives")
     if not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor")
     return t
@@ -95,13 +98,21 @@ def _tiled(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
     return t, rows, cols, ld
 
 
-def _pair(p, what: str):
-    """(q, scales, rows, cols, pitch) of a block-128 pair."""
+def _constant(p, what: str):
+    """The pair's two tensors, checked to want no derivative."""
     if not isinstance(p, (tuple, list)) or len(p) != 2:
         raise TypeError(f"{what} must be a (q, scales) pair")
     q, scales = p
     _on_gpu(q, what)
     _on_gpu(scales, what)
+    if (q.requires_grad or scales.requires_grad) and torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, and a pair has none: detach() it, or call under no_grad()")
+    return q, scales
+
+
+def _pair(p, what: str):
+    """(q, scales, rows, cols, pitch) of a block-128 pair."""
+    q, scales = _constant(p, what)
     if q.dtype != _FP8:
         raise ValueError(f"{what}: q must be float8_e4m3fn; got {q.dtype}")
     if scales.dtype != torch.float32:
@@ -187,6 +198,7 @@ def linear(x: torch.Tensor, weight, bias: Optional[torch.Tensor] = None,
             raise ValueError("linear with gradients needs bfloat16 activations")
         if isinstance(weight, torch.Tensor):
             return _Linear.apply(x, weight, bias, None)
+        _constant(weight, "weight")  # here, since the pass itself runs without gradients
         return _Linear.apply(x, None, bias, weight)
     return _forward(x, weight, bias, out_dtype, False)[0]
 
