@@ -243,7 +243,7 @@ cudaError_t dequantize_block128(Block128In in, MatOut x, FloatType type, int64_t
     Shape sh;
     if (!make_shape(rows, cols, 160, &sh) || !type_ok(type)) return cudaErrorInvalidValue;
     if (sh.total == 0) return cudaSuccess;
-    if (!mat_ok(x.ptr, x.ld, cols) || !q_ok(in.q, u32(in.ld), in.scales, cols)) return cudaErrorInvalidValue;
+    if (!mat_ok(x.ptr, x.ld, cols) || !q_ok(in.q, in.ld, in.scales, cols)) return cudaErrorInvalidValue;
     by_type(type, [&](auto t) {
         using T = decltype(t);
         auto* fn = vec_ok(x.ptr, x.ld, type) ? k_dequantize<T, true> : k_dequantize<T, false>;
@@ -259,7 +259,7 @@ cudaError_t swiglu_forward(MatIn gate, MatIn up, FloatType type, MatOut h, Block
     if (!make_shape(rows, cols, 160, &sh) || !type_ok(type)) return cudaErrorInvalidValue;
     if (sh.total == 0) return cudaSuccess;
     if (!mat_ok(gate.ptr, gate.ld, cols) || !mat_ok(up.ptr, up.ld, cols) || !mat_ok(h.ptr, h.ld, cols) ||
-        !q_ok(kg.q, u32(kg.ld), kg.scales, cols) || !q_ok(ku.q, u32(ku.ld), ku.scales, cols))
+        !q_ok(kg.q, kg.ld, kg.scales, cols) || !q_ok(ku.q, ku.ld, ku.scales, cols))
         return cudaErrorInvalidValue;
     const bool vec = vec_ok(gate.ptr, gate.ld, type) && vec_ok(up.ptr, up.ld, type) && vec_ok(h.ptr, h.ld, type);
     by_type(type, [&](auto t) {
@@ -278,7 +278,7 @@ cudaError_t swiglu_backward(MatIn dh, FloatType type, Block128In kg, Block128In 
     if (!make_shape(rows, cols, 20, &sh) || !type_ok(type)) return cudaErrorInvalidValue;
     if (sh.total == 0) return cudaSuccess;
     if (!mat_ok(dh.ptr, dh.ld, cols) || !mat_ok(dg.ptr, dg.ld, cols) || !mat_ok(du.ptr, du.ld, cols) ||
-        !q_ok(kg.q, u32(kg.ld), kg.scales, cols) || !q_ok(ku.q, u32(ku.ld), ku.scales, cols))
+        !q_ok(kg.q, kg.ld, kg.scales, cols) || !q_ok(ku.q, ku.ld, ku.scales, cols))
         return cudaErrorInvalidValue;
     const bool vec = vec_ok(dh.ptr, dh.ld, type) && vec_ok(dg.ptr, dg.ld, type) && vec_ok(du.ptr, du.ld, type);
     by_type(type, [&](auto t) {

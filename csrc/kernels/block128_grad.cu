@@ -802,8 +802,8 @@ cudaError_t choose(MatIn dy, int64_t dy_rows, int64_t dy_cols, const Block128In&
 
 bool args_ok(const MatIn& dy, int64_t n, const Block128In& q, const MatOut& out, int64_t k, FloatType type) {
     auto aligned = [](const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-    return aligned(dy.ptr) && dy.ld >= n && dy.ld % 8 == 0 && aligned(q.q) && q.scales && q.ld % 16 == 0 &&
-           q.ld >= k && out.ptr && out.ld >= k && int(type) >= 0 && int(type) <= 2;
+    return aligned(dy.ptr) && dy.ld >= n && dy.ld % 8 == 0 && dy.ld < kMostPitch / 2 && aligned(q.q) && q.scales &&
+           q.ld % 16 == 0 && q.ld >= k && q.ld < kMostPitch && out.ptr && out.ld >= k && int(type) >= 0 && int(type) <= 2;
 }
 bool work_ok(const GradWork& w) { return reinterpret_cast<uintptr_t>(w.words) % 4 == 0; }
 bool dims_ok(int64_t a, int64_t b, int64_t c) {

@@ -12,6 +12,8 @@ namespace kern {
 
 extern std::atomic<uint64_t> g_block128_launches;
 
+constexpr int64_t kMostPitch = int64_t(1) << 40;  // bytes: a tensor map's pitch is below this
+
 // Tensor map of a row-major [rows, cols] matrix with `pitch` bytes a row, read
 // in tiles of box_rows x box_cols in a swizzle of 128, 64 or 0
 // bytes; what lies outside reads as 0.

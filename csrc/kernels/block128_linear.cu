@@ -399,7 +399,8 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
 }
 
 bool q_ok(const Block128In& t, int64_t cols) {
-    return t.q && t.scales && (reinterpret_cast<uintptr_t>(t.q) & 15) == 0 && t.ld % 16 == 0 && t.ld >= cols;
+    return t.q && t.scales && (reinterpret_cast<uintptr_t>(t.q) & 15) == 0 && t.ld % 16 == 0 && t.ld >= cols &&
+           t.ld < kMostPitch;
 }
 
 struct Problem {
@@ -498,7 +499,8 @@ cudaError_t linear_block128(MatIn x, FloatType xtype, Block128Out kept, void* wo
         return cudaErrorInvalidValue;
     if (m == 0) return cudaSuccess;
     if (n == 0) return kept.scales ? quantize_block128(x, xtype, kept, m, k, s) : cudaSuccess;
-    if (!x.ptr || x.ld < k || int(xtype) < 0 || int(xtype) > 2 || !q_ok(w, k) || !y.ptr || y.ld < n || !work ||
+    if (!x.ptr || x.ld < k || x.ld > 0xffffffff || kept.ld < k || kept.ld % 16 != 0 || kept.ld >= kMostPitch ||
+        !kept.q || int(xtype) < 0 || int(xtype) > 2 || !q_ok(w, k) || !y.ptr || y.ld < n || !work ||
         (reinterpret_cast<uintptr_t>(work) & 15))
         return cudaErrorInvalidValue;
     const Problem p{x, xtype, kept, static_cast<uint32_t*>(work), work_bytes, w, bias, y, type, m, n, k, s};
