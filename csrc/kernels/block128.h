@@ -80,6 +80,8 @@ uint64_t block128_launch_count();
 // `device` (its result is then incomplete); 0 if none did. Host memory, read
 // without waiting for the device.
 uint32_t block128_error(int device);
+// Sets that word (0: it has been dealt with). No effect before a product has run on the device.
+void block128_set_error(int device, uint32_t code);
 
 }  // namespace kern
 }  // namespace ofld

@@ -111,6 +111,11 @@ uint32_t block128_error(int device) {
     return *static_cast<volatile uint32_t*>(g_dev[device].host);
 }
 
+void block128_set_error(int device, uint32_t code) {
+    if (device < 0 || device >= kDevices || !g_ready[device].load(std::memory_order_acquire)) return;
+    *static_cast<volatile uint32_t*>(g_dev[device].host) = code;
+}
+
 cudaError_t allow_smem(const void* fn, uint32_t bytes) {
     static std::mutex mu;
     static std::set<std::pair<const void*, int>> done;

@@ -1,9 +1,10 @@
 // Thin wrappers of the sm_100a instructions that the product kernels use:
 // mbarriers, tiled bulk copies, clusters, tensor memory and tcgen05.
 //
-// Every wait is bounded. One that runs out stores a code in the launch's
-// error word and raises the CTA's abort flag, which ends the waits of the
-// other warps too, so that the kernel returns and the host sees the code.
+// Every wait on an mbarrier is bounded. One that runs out stores a code in the
+// launch's error word and raises the CTA's abort flag, which ends the waits of
+// the other warps too, so that the kernel returns and the host can see the
+// code. Barriers of the CTA and the cluster, which all warps reach, are not.
 #pragma once
 
 #include <cuda.h>

@@ -13,14 +13,15 @@ void check(cudaError_t e, const char* what) {
     if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
 }
 // A product kernel whose bounded wait ran out has left its result incomplete:
-// the calls after it say so.
+// the products launched after it say so, until the word is cleared.
 void check_product(cudaError_t e, const char* what) {
     check(e, what);
     int dev = -1;
     if (cudaGetDevice(&dev) != cudaSuccess) return;  // nothing can have been launched
     if (const uint32_t code = block128_error(dev))
         throw std::runtime_error(std::string(what) + ": a product on this device gave up waiting (code " +
-                                 std::to_string(code) + "); results since then are not complete");
+                                 std::to_string(code) +
+                                 "); results since then are not complete. ops.product_error tells and clears it");
 }
 MatIn in(uint64_t p, int64_t ld) { return {reinterpret_cast<const void*>(p), ld}; }
 MatOut out(uint64_t p, int64_t ld) { return {reinterpret_cast<void*>(p), ld}; }
@@ -36,6 +37,7 @@ cudaStream_t stream(uint64_t s) { return reinterpret_cast<cudaStream_t>(s); }
 
 void bind_block128(py::module_& m) {
     m.def("block128_error", &block128_error);
+    m.def("block128_set_error", &block128_set_error);
     m.def("k_quantize_block128", [](uint64_t x, int64_t ldx, int type, uint64_t q, int64_t ldq, uint64_t sc,
                                     int64_t rows, int64_t cols, uint64_t s) {
         check(quantize_block128(in(x, ldx), FloatType(type), qout(q, ldq, sc), rows, cols, stream(s)),

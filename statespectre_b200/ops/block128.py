@@ -294,6 +294,19 @@ def linear_weight_grad(dy: torch.Tensor, x: Block128, out_dtype: torch.dtype = t
     return dw
 
 
+def product_error(device=None, clear: bool = False) -> int:
+    """0, or the code of the first product on ``device`` (the current one) whose bounded wait for a tile ran out, which
+    leaves its result incomplete. Products launched later raise ``RuntimeError`` for it; a replayed graph and work that
+    is still running cannot, so ask after a synchronization. ``clear`` ends the raising."""
+    index = None if device is None else torch.device(device).index if not isinstance(device, int) else device
+    if index is None:
+        index = torch.cuda.current_device()
+    code = native().block128_error(index)
+    if clear and code:
+        native().block128_set_error(index, 0)
+    return code
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, pair):
