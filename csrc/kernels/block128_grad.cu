@@ -115,6 +115,7 @@ struct Config {
     static constexpr uint32_t off_scale = off_out + 4 * 2 * out_bytes;
     static constexpr uint32_t off_bar = off_scale + NQ * kStep * 4;
     static constexpr uint32_t off_misc = off_bar + (2 * (NA + NQ + NB) + 4) * 8;
+    static_assert(off_misc % 8 == 0, "a barrier there");
     static constexpr uint32_t smem = off_misc + 16 + 1024;
     static constexpr uint32_t tmem_cols = 2 * BN;
     static_assert(smem <= 227 * 1024 && tmem_cols <= 512, "");
@@ -258,7 +259,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto b_empty = [&](uint32_t s) { return bar + 8 * (2 * (C::NA + C::NQ) + C::NB + s); };
     auto tfull = [&](uint32_t b) { return bar + 8 * (2 * (C::NA + C::NQ + C::NB) + b); };
     auto tempty = [&](uint32_t b) { return bar + 8 * (2 * (C::NA + C::NQ + C::NB) + 2 + b); };
-    volatile uint32_t* const misc = reinterpret_cast<volatile uint32_t*>(sm + C::off_misc);  // tensor memory, abort
+    // tensor memory, abort, a barrier for the end of an aborted launch
+    volatile uint32_t* const misc = reinterpret_cast<volatile uint32_t*>(sm + C::off_misc);
+    const uint32_t drained = base + C::off_misc + 8;
     const Guard guard{misc + 1, a.error};
 
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
@@ -286,6 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t s = 0; s < C::NQ; ++s) mbar_init(q_full(s), 1 + 32), mbar_init(q_empty(s), kGroupWarps);
         for (uint32_t s = 0; s < C::NB; ++s) mbar_init(b_full(s), kGroupWarps * C::CG), mbar_init(b_empty(s), 1);
         for (uint32_t b = 0; b < 2; ++b) mbar_init(tfull(b), 1), mbar_init(tempty(b), 4 * C::CG);
+        mbar_init(drained, 1);
         mbar_init_fence();
         misc[1] = 0;
     }
@@ -405,12 +409,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
+            if (*guard.abort && leader) mma_drain<C::CG>(drained);
         };
         if (half == 0) {
             if (__builtin_expect(odd, 0))
                 issue(std::true_type{});
             else
                 issue(std::false_type{});
+            __syncwarp();
         }
     } else if (warp == 2) {
         const bool leader = elect_one();

@@ -85,6 +85,7 @@ struct Config {
     static constexpr uint32_t tmem_cols = tmem_used <= 64 ? 64 : tmem_used <= 128 ? 128 : tmem_used <= 256 ? 256 : 512;
     static constexpr uint32_t off_bar = ST * stage_pitch;
     static constexpr uint32_t off_misc = off_bar + (2 * ST + 2 * NBUF) * 8;
+    static_assert(off_misc % 8 == 0, "a barrier there");
     static constexpr uint32_t smem = off_misc + 16 + 1024;  // + alignment of the base
     static constexpr int CPT = BN / (EW / 4);                  // columns of one epilogue thread
     static constexpr int CH = CPT % 32 ? 16 : 32;            // columns of one tensor-memory load
@@ -152,7 +153,9 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
     auto empty = [&](uint32_t s) { return bar + 8 * (C::ST + s); };
     auto tfull = [&](uint32_t b) { return bar + 8 * (2 * C::ST + b); };
     auto tempty = [&](uint32_t b) { return bar + 8 * (2 * C::ST + C::NBUF + b); };
-    volatile uint32_t* const misc = reinterpret_cast<volatile uint32_t*>(sm + C::off_misc);  // tensor memory, abort
+    // tensor memory, abort, a barrier for the end of an aborted launch
+    volatile uint32_t* const misc = reinterpret_cast<volatile uint32_t*>(sm + C::off_misc);
+    const uint32_t drained = base + C::off_misc + 8;
     const Guard guard{misc + 1, a.error};
 
     // one value for a warp, so that what the issuing warps compute stays in uniform registers
@@ -168,6 +171,7 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < C::ST; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
         for (uint32_t b = 0; b < C::NBUF; ++b) mbar_init(tfull(b), 1), mbar_init(tempty(b), C::EW * C::CG);
+        mbar_init(drained, 1);
         mbar_init_fence();
         misc[1] = 0;
     }
@@ -295,6 +299,8 @@ __global__ void __launch_bounds__(C::threads, C::per_sm)
                     if (++s == C::ST) s = 0, sphase ^= 1;
                     if (++b == C::NBUF) b = 0, bphase ^= 1;
                 }
+            if (*guard.abort && leader) mma_drain<C::CG>(drained);
+            __syncwarp();
         }
         // Even shares of registers again, for the code that all warps run; not
         // before every warp is done with its own.

@@ -268,6 +268,18 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
             : "memory");
 }
 
+// After a wait that ran out: the thread that issued products and copies to
+// tensor memory waits (with a limit) for those in flight, which read shared
+// memory and write tensor memory that the block is about to give back. `bar`
+// is a barrier of one arrival that nothing else uses.
+template <int CG>
+__device__ __forceinline__ void mma_drain(uint32_t bar) {
+    mma_commit<CG>(bar);
+    const long long t0 = clock64();
+    while (!mbar_test(bar, 0) && clock64() - t0 < kWaitCycles / 8) {
+    }
+}
+
 #define OFLD_W4(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
 #define OFLD_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
 
