@@ -75,8 +75,7 @@ def _matrix(t: torch.Tensor, what: str) -> Tuple[torch.Tensor, int, int, int]:
     if t.dim() != 2:
         if t.dim() == 0:
             raise ValueError(f"{what} must have at least one dimension")
-        cols = t.shape[-1]
-        t = t.reshape(t.numel() // cols if cols else 0, cols)
+        t = t.reshape(t.shape[:-1].numel(), t.shape[-1])
     rows, cols = t.shape
     pitch, one = t.stride()
     if (cols > 1 and one != 1) or (rows > 1 and not cols <= pitch < _MOST):
@@ -329,7 +328,7 @@ class _Linear(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             dw = linear_weight_grad(dy, (xq, xs), ctx.weight_dtype)
         if ctx.needs_input_grad[2]:
-            db = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32).to(ctx.bias_dtype)
+            db = dy.reshape(dy.shape[:-1].numel(), dy.shape[-1]).sum(0, dtype=torch.float32).to(ctx.bias_dtype)
         return dx, dw, db, None
 
 

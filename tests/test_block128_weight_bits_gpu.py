@@ -106,3 +106,62 @@ def test_gradient_at_the_weights_that_the_product_saw():
     ref = dy.double() @ values(w)
     assert (dx.double() - ref).norm() <= 1.01 * (ref.to(BF16).double() - ref).norm()
     assert half_step(BF16) == 2.0 ** -8
+
+
+def test_captured_gradients_follow_their_scales():
+    """The kind of a pair's scales is found as the work runs: graphs that replay side by side, in pairs of CTAs and in
+    single ones, give what eager calls give as powers of two turn into other scales and back."""
+    cases = [(randn((1300, 520), 1), amax_pair(520, 1500, 2)), (randn((70, 900), 3), amax_pair(900, 300, 4)),
+             (randn((600, 1400), 5), amax_pair(1400, 2600, 6))]
+    both = [(s, 2.0 ** torch.floor(torch.log2(s))) for _, (_, s) in cases]
+    both = [(a.clone(), b) for a, b in both]
+
+    def step():
+        return [ops.linear_input_grad(dy, w, out) for dy, w in cases for out in (BF16, FP32)]
+
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out, torch.cuda.Stream()))
+    for turn in range(6):
+        for (_, w), kinds in zip(cases, both):
+            w[1].copy_(kinds[turn % 2])
+        want = step()
+        for g, _, s in graphs:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        for _, out, s in graphs:
+            torch.cuda.current_stream().wait_stream(s)
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+    i = 0
+    for dy, w in cases:
+        for out in (BF16, FP32):
+            check_product(want[i], dy.double(), values(w), out, dy.shape[1], off(out))
+            i += 1
+
+
+def test_pairs_of_several_threads():
+    import threading
+
+    data = [(randn((700 + 200 * i, 300 + 64 * i), i), amax_pair(300 + 64 * i, 2600, i + 9)) for i in range(3)]
+    want = [ops.linear_input_grad(*d) for d in data]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                got = ops.linear_input_grad(*data[i])
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(got, want[i]):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(len(data))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
