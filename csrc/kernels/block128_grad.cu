@@ -29,8 +29,8 @@
 // tensor core spends 512 cycles on the step before. Few outputs: one CTA owns
 // 128 x 128, and the sum is split over a cluster of up to 8.
 //
-// 8192 tokens, 14336 x 4096, bf16 results: 669 us (1.44 PFLOP/s, the tensor
-// pipe active 77 % of the cycles; cuBLAS bf16 reaches 1.65 in bursts and 1.38
+// 8192 tokens, 14336 x 4096, bf16 results: 670 us (1.44 PFLOP/s, the tensor
+// pipe active 76 % of the cycles; cuBLAS bf16 reaches 1.65 in bursts and 1.38
 // in a loop of seconds, under the power cap that bounds this kernel too). What
 // it took: a converter that arrives without a release to the cluster (746 us
 // to 357 for 4096 x 4096 x 14336), a ring for each kind of tile, and results
@@ -84,7 +84,7 @@ enum : uint32_t {
     kWaitTmemFull
 };
 
-constexpr uint32_t kOddThreads = 256;
+constexpr uint32_t kOddThreads = 1024;
 
 struct Args {
     const float* scales;
