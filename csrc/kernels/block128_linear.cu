@@ -22,11 +22,12 @@
 //
 // Many tokens: a pair of CTAs owns 256 x 224 results. A block of the sum takes
 // the tensor core 448 cycles and the epilogue 112 multiply-adds a lane, 224
-// issue slots of each scheduler. 4096 x 5120 x 27648: 526 us (2.2 PFLOP/s), 650
-// in a loop of seconds. A block takes about 800 cycles: the issuing warp needs
-// 600 of them (two in turn were no faster), the epilogue 620. At 1000 W the SMs
-// run at 1.6 GHz; without the epilogue's arithmetic they run at 1.48 GHz and
-// need 416 us, so the power cap would take most of what fewer cycles gave.
+// issue slots of each scheduler. 4096 x 5120 x 27648: 540 us (2.1 PFLOP/s); with
+// x's quantisation 567, in a loop of seconds 666. A block takes about 800
+// cycles: the issuing warp is busy for 690 of them (two in turn were no
+// faster), the epilogue for all. At 1000 W the SMs run at 1.6 GHz; without the
+// epilogue's arithmetic they run at 1.48 GHz and need 416 us, so the power cap
+// would take most of what fewer cycles gave.
 // Few tokens: the bytes of w, in tiles of 128 rows x 16, 32 or 64 tokens, the
 // sum in parts over a cluster. 16 tokens x 4096 x 14336: 14.9 us (4 TB/s), one
 // token x 5120 x 5120: 10.2 us, of which 3 to 4 are starting and joining.

@@ -29,7 +29,7 @@ import torch
 from .._native import native
 
 
-def _operator(name: str, shape: str, iters: int) -> None:
+def _operator(name: str, shape: str, iters: int, scales: str) -> None:
     from . import dequantize, linear, linear_input_grad, linear_weight_grad, quantize, swiglu_backward, swiglu_forward
 
     m, n, k = (int(v) for v in shape.split(","))
@@ -38,15 +38,19 @@ def _operator(name: str, shape: str, iters: int) -> None:
     def rand(rows, cols, std=1.0):
         return (torch.randn(rows, cols, device=dev) * std).to(torch.bfloat16)
 
+    def pair(rows, cols, std=1.0):
+        q, s = quantize(rand(rows, cols, std))
+        return q, s if scales == "pow2" else s * 1.37
+
     flops, moved = 2 * m * n * k, 0
     if name == "linear":
-        x, w = rand(m, k), quantize(rand(n, k, 0.02))
+        x, w = rand(m, k), pair(n, k, 0.02)
         run = lambda: linear(x, w)  # noqa: E731
     elif name == "input_grad":
-        dy, w = rand(m, n), quantize(rand(n, k, 0.02))
+        dy, w = rand(m, n), pair(n, k, 0.02)
         run = lambda: linear_input_grad(dy, w)  # noqa: E731
     elif name == "weight_grad":
-        dy, x = rand(m, n), quantize(rand(m, k))
+        dy, x = rand(m, n), pair(m, k)
         run = lambda: linear_weight_grad(dy, x)  # noqa: E731
     else:
         flops, moved = 0, m * k * (16 if name == "swiglu" else 6)
@@ -80,6 +84,8 @@ def main():
                                                           "evict_zf32", "restore_zf32", "evict_zf32_stage",
                                                           "restore_zf32_stage", *OPERATORS])
     ap.add_argument("--shape", default="2048,4096,9472", help="operators: tokens, outputs, inputs")
+    ap.add_argument("--scales", choices=["pow2", "any"], default="pow2",
+                    help="products: powers of two, as quantize makes them, or others, as pushed weights have")
     ap.add_argument("--mb", type=int, default=512)
     ap.add_argument("--iters", type=int, default=3)
     ap.add_argument("--ctas", type=int, default=0)
@@ -92,7 +98,7 @@ def main():
                          "(every chunk stored after its digest), 2 = delta mode with nothing changed")
     a = ap.parse_args()
     if a.kernel in OPERATORS:
-        _operator(a.kernel, a.shape, a.iters)
+        _operator(a.kernel, a.shape, a.iters, a.scales)
         return
     C = native()
     n = a.mb << 20
