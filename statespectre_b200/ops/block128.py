@@ -109,6 +109,17 @@ def _constant(p, what: str):
     return q, scales
 
 
+def _row_wise(shape, rows: int, cols: int) -> bool:
+    """Whether as many scales as there are blocks lie row by row in this shape: its last dimensions make up a row, or it
+    is flat. Flat scales count on from one row to the next, which is the same where rows end on a block."""
+    blocks, n = -(-cols // BLOCK), 1
+    for d in reversed(shape):
+        n *= d
+        if n == blocks:
+            return True
+    return n == 0 or ((rows == 1 or cols % BLOCK == 0) and max(shape, default=1) == n)
+
+
 def _pair(p, what: str):
     """(q, scales, rows, cols, pitch) of a block-128 pair."""
     q, scales = _constant(p, what)
@@ -119,10 +130,7 @@ def _pair(p, what: str):
     _same_device(q, scales, what)
     q, rows, cols, ld = _tiled(q, what)
     blocks = -(-cols // BLOCK)
-    count = scales.numel()
-    last = scales.shape[-1] if scales.dim() else 0
-    # Flat scales (count == last) count on from one row to the next, which is the same where rows end on a block.
-    if count != rows * blocks or (count and last != blocks and (count != last or (rows > 1 and cols % BLOCK))):
+    if scales.numel() != rows * blocks or not (scales.shape[-1:] == (blocks,) or _row_wise(scales.shape, rows, cols)):
         raise ValueError(f"{what}: {tuple(scales.shape)} scales do not fit {rows} rows of {cols} values: one for "
                          f"each {BLOCK} values of a row, flat only where rows are multiples of {BLOCK}")
     return q, scales if scales.is_contiguous() else scales.contiguous(), rows, cols, ld

@@ -36,15 +36,18 @@ def test_scales_that_run_on_across_rows_are_refused(any_device, rows, cols, call
         call((q(rows, cols), scales))
 
 
-@pytest.mark.parametrize("shape,scales", [((8, 256), (2, 8)), ((8, 256), (8, 2, 1)), ((8, 200), (16,)),
-                                          ((8, 200), (1, 16)), ((3, 20, 200), (120,)), ((3, 20, 256), (3, 2, 20)), ((6, 127), (1, 6))])
+@pytest.mark.parametrize("shape,scales", [((8, 256), (2, 8)), ((8, 200), (16,)),
+                                          ((8, 200), (1, 16)), ((3, 20, 200), (120,)), ((3, 20, 256), (3, 2, 20)),
+                                          ((6, 127), (1, 6))])
 def test_scales_of_another_shape_are_refused(any_device, shape, scales):
     with pytest.raises(ValueError, match="do not fit"):
         ops.dequantize((q(*shape), torch.ones(scales)))
 
 
-@pytest.mark.parametrize("shape,scales", [((8, 256), (8, 2)), ((8, 256), (16,)), ((8, 256), (1, 16)), ((8, 200), (8, 2)),
-                                          ((1, 200), (2,)), ((200,), (2,)), ((3, 20, 200), (3, 20, 2)), ((3, 20, 200), (60, 2)),
+@pytest.mark.parametrize("shape,scales", [((8, 256), (8, 2)), ((8, 256), (16,)), ((8, 256), (1, 16)), ((8, 256), (16, 1)),
+                                          ((8, 256), (8, 2, 1)), ((8, 200), (8, 2, 1)), ((8, 200), (8, 2)), ((1, 100), ()),
+                                          ((1, 200), (2,)), ((200,), (2,)), ((3, 20, 200), (3, 20, 2)),
+                                          ((3, 20, 200), (60, 2)),
                                           ((60, 200), (3, 20, 2)), ((3, 20, 256), (120,)), ((6, 127), (6, 1)),
                                           ((0, 200), (0, 2)), ((0, 200), (0,)), ((5, 0), (5, 0)), ((1, 1, 200), (2,))])
 def test_scales_that_fit(any_device, shape, scales):
