@@ -47,3 +47,9 @@ def test_product_pitches_are_refused(name, bad):
             C.k_matmul_input_grad(A, p["x"], A, p["w"], A, A, p["y"], 0, 4, 256, 256, 0)
         with pytest.raises(RuntimeError, match="invalid argument"):
             C.k_matmul_weight_grad(A, p["x"], A, p["w"], A, A, p["y"], 0, 4, 256, 256, 0)
+
+
+def test_words_of_a_gradient_are_whole():
+    for fn in (native().k_matmul_input_grad, native().k_matmul_weight_grad):
+        with pytest.raises(RuntimeError, match="invalid argument"):
+            fn(A, 256, A, 256, A, A, 256, 0, 4, 256, 256, 0, work=A + 2, words=148)
